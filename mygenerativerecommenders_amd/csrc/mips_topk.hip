@@ -510,7 +510,8 @@ __device__ __forceinline__ void mips_select_unit(const SelectArgs& a, const int 
   };
   auto process = [&](const fv2 (&f)[BLOCKS][KS2], int step) {
     const float tau = tau_s[lr];
-    const int64_t xb = x_begin + ((int64_t)step * SW + w) * STEP;
+    // items of this step as 32-bit indices (X < 2^31): the registers are full at KS = 64
+    const int xb = (int)(x_begin + ((int64_t)step * SW + w) * STEP);
     f4 s[BLOCKS];
 #pragma unroll
     for (int bb = 0; bb < BLOCKS; ++bb) s[bb] = f4_zero();
@@ -523,11 +524,11 @@ __device__ __forceinline__ void mips_select_unit(const SelectArgs& a, const int 
     for (int bb = 0; bb < BLOCKS; ++bb) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int64_t item = xb + bb * 16 + 4 * lg + r;
-        if (item < x_end && s[bb][r] > tau) {
+        const uint32_t item = (uint32_t)(xb + bb * 16 + 4 * lg + r);
+        if (item < (uint32_t)x_end && s[bb][r] > tau) {
           const int slot = atomicAdd(&cnt[lr], 1);
           cs[lr * CAP + slot] = s[bb][r];
-          ci[lr * CAP + slot] = (uint32_t)item;  // local index
+          ci[lr * CAP + slot] = item;  // local index
         }
       }
     }
