@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define GR_HSTU_ABI_VERSION 18
+#define GR_HSTU_ABI_VERSION 19
 
 #ifndef GR_API
 #define GR_API __attribute__((visibility("default")))
@@ -47,7 +47,8 @@ GR_API int gr_version(void);
  * wgrad_reduce, mips_pack, mips_select, mips_merge, cumsum, dense_to_jagged, encoder_prologue, bf16_scale_add, adamw,
  * jagged_to_padded, l2_normalize, current_embeddings, sampled_softmax_fwd,
  * sampled_softmax_bwd, sampled_softmax_csr, sampled_softmax_table_grad, preproc, rows_copy,
- * decode_scatter, decode_attn, softmax_attn_fwd, softmax_attn_bwd, rel_bias_fwd, rel_bias_bwd.  Not for use inside a captured graph.
+ * decode_scatter, decode_attn, softmax_attn_fwd, softmax_attn_bwd, rel_bias_fwd, rel_bias_bwd,
+ * adamw8, layer_norm_fwd, layer_norm_bwd, jagged_attn_fwd, jagged_attn_bwd.  Not for use inside a captured graph.
  */
 GR_API int gr_timing_enable(int on);
 GR_API int gr_timing_query(const char* kernel, double* total_ms, int* launches);
@@ -275,6 +276,68 @@ GR_API int gr_adamw_step(float* const* params, const float* const* grads, const 
                          const int64_t* numel, int n_tensors, float* exp_avg, float* exp_avg_sq,
                          float* step, uint32_t* done, double lr, double beta1, double beta2,
                          double eps, double weight_decay, void* stream);
+
+/* gr_adamw8_step (ABI 19): the same update with both moments held in 8 bits: an OCP e4m3
+ * code per element (exp_avg / exp_avg_sq) times a power-of-two fp32 scale per 64 elements of
+ * a tensor (exp_avg_scale / exp_avg_sq_scale, entry e of the moments under scale e / 64).
+ * offs must be multiples of 64, and a tensor's moments are padded to a multiple of 64 (the
+ * padding codes are zero and stay zero).  The parameter moves by the new moments before
+ * they are rounded; each is rounded down or up at random, by 20 bits of a hash of
+ * (offs[i] + element, step), with the probability of its place between its neighbours, and a
+ * nonzero exp_avg_sq never becomes zero.  A block that holds an infinity or NaN gets a NaN
+ * scale.  Hyper-parameters are rounded once to fp32 (1 - beta, 1 - lr wd from doubles), the
+ * bias corrections computed in double.  One launch per 64 tensors; step and done as above. */
+GR_API int gr_adamw8_step(float* const* params, const float* const* grads, const int64_t* offs,
+                          const int64_t* numel, int n_tensors, uint8_t* exp_avg,
+                          float* exp_avg_scale, uint8_t* exp_avg_sq, float* exp_avg_sq_scale,
+                          float* step, uint32_t* done, double lr, double beta1, double beta2,
+                          double eps, double weight_decay, void* stream);
+
+/* ---------------------------------------------------------------- layer norm (ABI 19)
+ * Rows of D elements, row strides ld_* in elements (>= D, or 0 for one row read for all),
+ * no alignment beyond the element's.  types: bit 0: x, y, dy, dx are bf16 (else fp32);
+ * bit 1: weight, bias and their gradients are bf16 (else fp32).  weight / bias may be NULL.
+ * Forward: y = (x - mu) r weight + bias with mu, r = 1 / sqrt(var + eps) of each row (var
+ * over D, from centred values), sums in fp32; stats (rows, 2) receives (mu, r) unless NULL
+ * (the backward needs it).
+ * Backward: dx (NULL: not wanted), dweight = sum_rows dy xh, dbias = sum_rows dy (NULL: not
+ * wanted) in a fixed order; the workspace (gr_layer_norm_bwd_workspace_size bytes) is only
+ * read or written when one of the two is wanted.  y / dx must not alias the inputs. */
+GR_API int gr_layer_norm_fwd(const void* x, int64_t ld_x, int64_t rows, int D, const void* weight,
+                             const void* bias, int types, float eps, void* y, int64_t ld_y,
+                             float* stats, void* stream);
+GR_API size_t gr_layer_norm_bwd_workspace_size(int64_t rows, int D, int types);
+GR_API int gr_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x,
+                             int64_t rows, int D, const void* weight, int types,
+                             const float* stats, void* dx, int64_t ld_dx, void* dweight,
+                             void* dbias, void* workspace, size_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------- jagged attention (ABI 19)
+ * Softmax attention of each head over the rows of its own sequence (rows offsets[b] ..
+ * offsets[b + 1]), keys j <= i only where causal:
+ *   out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h']) v[j, h'],  h' = h / (H / Hkv)
+ * q (rows, H, d), k (rows, Hkv, d), v (rows, Hkv, dv): bf16 (bf16 != 0) or fp32, element
+ * strides ld_* of a row and hs_* of a head, columns contiguous, no alignment beyond the
+ * element's; 1 <= d, dv <= 256, H a multiple of Hkv, scale > 0.  out, dout (rows, H, dv), dq
+ * (rows, H, d), dk (rows, Hkv, d), dvv (rows, Hkv, dv) are contiguous.  Rows past
+ * offsets[B] get zeros; offsets are clamped to [0, rows].  lse (H, rows): log2 of each row's
+ * sum of exp(scaled scores), which the backward needs (forward: NULL if there is none).
+ * The backward recomputes the probabilities; dk / dvv sum over the heads that share them.
+ * Accumulation and softmax in fp32; no atomics, the same bits every run.  Workspace:
+ * gr_jagged_attn_bwd_workspace_size bytes. */
+GR_API int gr_jagged_attn_fwd(const void* q, int64_t ld_q, int64_t hs_q, const void* k,
+                              int64_t ld_k, int64_t hs_k, const void* v, int64_t ld_v,
+                              int64_t hs_v, const int64_t* offsets, int B, int64_t rows, int H,
+                              int Hkv, int d, int dv, int causal, float scale, int bf16,
+                              void* out, float* lse, void* stream);
+GR_API size_t gr_jagged_attn_bwd_workspace_size(int64_t rows, int H);
+GR_API int gr_jagged_attn_bwd(const void* q, int64_t ld_q, int64_t hs_q, const void* k,
+                              int64_t ld_k, int64_t hs_k, const void* v, int64_t ld_v,
+                              int64_t hs_v, const int64_t* offsets, int B, int64_t rows, int H,
+                              int Hkv, int d, int dv, int causal, float scale, int bf16,
+                              const void* out, const float* lse, const void* dout, void* dq,
+                              void* dk, void* dvv, void* workspace, size_t ws_bytes,
+                              void* stream);
 
 /* ---------------------------------------------------------------- HSTU attention
  * hstu_bucket_map: the relative-time bucket of every causal (query i, key j) pair of

@@ -12,11 +12,15 @@ Reference map (``src/generative_recommenders_pl/models/``):
   * sampled_softmax_loss ......... losses/autoregressive_losses.py:259-306 (+ the
                                    negatives gather of negative_sampler.py:105-131)
   * STU layer fwd/bwd ............ sequential_encoders/hstu.py:266-413 (+ autograd)
+  * layer_norm ................... postprocessors/postprocessors.py:59-80 (and affine)
+  * jagged_attention ............. no counterpart: per-head softmax attention, jagged rows
 """
 from __future__ import annotations
 
 
+import contextlib
 import ctypes
+import math
 from dataclasses import dataclass
 from typing import Optional
 
@@ -185,6 +189,101 @@ def l2_normalize(x: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
     if x.dtype != torch.float32:
         raise TypeError("l2_normalize: float32 only")
     return _L2Normalize.apply(x, float(eps))
+
+
+# ------------------------------------------------------------------ layer norm
+
+_FLOATS = (torch.float32, torch.bfloat16)
+
+
+def _on(device):
+    """The device's own context where it is not the current one: launches and the current
+    stream then are that device's."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _rows_of(x, D: int):
+    """x as (rows, D) with contiguous columns: a view wherever its strides allow."""
+    x2 = x.reshape(-1, D)
+    return x2 if D == 1 or x2.stride(1) == 1 else x2.contiguous()
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps: float, grad_on: bool):
+        D = x.shape[-1]
+        x2 = _rows_of(x, D)
+        rows = x2.shape[0]
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device) if grad_on else None
+        affine = weight if weight is not None else bias
+        types = int(x.dtype == torch.bfloat16) + 2 * int(affine is not None and affine.dtype == torch.bfloat16)
+        with _on(x.device):
+            _lib.call("gr_layer_norm_fwd", x2.data_ptr(), x2.stride(0), rows, D, _lib.ptr(weight),
+                      _lib.ptr(bias), types, eps, y.data_ptr(), D, _lib.ptr(stats), _stream())
+        if grad_on:
+            ctx.save_for_backward(x, weight, bias, stats)
+        ctx.types, ctx.eps = types, eps
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, weight, bias, stats = ctx.saved_tensors
+        D = x.shape[-1]
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        if torch.is_grad_enabled():  # create_graph: differentiable torch operations
+            return (*_layer_norm_grads(x, weight, bias, ctx.eps, dy, want_x, want_w, want_b), None, None)
+        x2, g = _rows_of(x, D), _rows_of(dy, D)
+        rows = x2.shape[0]
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
+        dw = torch.empty_like(weight) if want_w else None
+        db = torch.empty_like(bias) if want_b else None
+        n = _lib.lib().gr_layer_norm_bwd_workspace_size(rows, D, ctx.types) if want_w or want_b else 0
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+        with _on(x.device):
+            _lib.call("gr_layer_norm_bwd", g.data_ptr(), g.stride(0), x2.data_ptr(), x2.stride(0), rows,
+                      D, _lib.ptr(weight), ctx.types, stats.data_ptr(), _lib.ptr(dx), D, _lib.ptr(dw),
+                      _lib.ptr(db), _lib.ptr(ws), n, _stream())
+        return dx, dw, db, None, None
+
+
+def _layer_norm_grads(x, weight, bias, eps, dy, want_x, want_w, want_b):
+    xf, g = x.float(), dy.float()
+    c = xf - xf.mean(-1, keepdim=True)
+    r = torch.rsqrt((c * c).mean(-1, keepdim=True) + eps)
+    xh = c * r
+    gw = g if weight is None else g * weight.float()
+    dx = r * (gw - gw.mean(-1, keepdim=True) - xh * (gw * xh).mean(-1, keepdim=True))
+    D = x.shape[-1]
+    return (dx.to(x.dtype) if want_x else None,
+            (g * xh).reshape(-1, D).sum(0).to(weight.dtype) if want_w else None,
+            g.reshape(-1, D).sum(0).to(bias.dtype) if want_b else None)
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension, forward and
+    backward (``gr_layer_norm_fwd`` / ``_bwd``; postprocessors.py:59-80 is the form without
+    weight and bias).  x is float32 or bfloat16 with any strides (a view whose rows have
+    one stride is read in place); weight and bias (D,), each optional, share one of the two
+    types.  Sums are fp32; the output has x's type, the weight's and bias's gradients are
+    summed over the rows in a fixed order."""
+    _lib.require_gpu(x, weight, bias)
+    if x.dtype not in _FLOATS:
+        raise TypeError("layer_norm: float32 or bfloat16 expected")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("layer_norm: a last dimension of at least one element expected")
+    params = [t for t in (weight, bias) if t is not None]
+    for t in params:
+        if t.dtype not in _FLOATS or t.dtype != params[0].dtype:
+            raise TypeError("layer_norm: weight and bias must be float32 or bfloat16, both the same")
+        if tuple(t.shape) != (x.shape[-1],) or t.device != x.device:
+            raise ValueError(f"layer_norm: weight and bias must be ({x.shape[-1]},) tensors on {x.device}")
+    grad_on = torch.is_grad_enabled() and any(t.requires_grad for t in (x, *params))
+    return _LayerNorm.apply(x, None if weight is None else weight.contiguous(),
+                            None if bias is None else bias.contiguous(), float(eps), grad_on)
 
 
 # ------------------------------------------------------------------ relative-time buckets
@@ -1183,6 +1282,87 @@ def stu_softmax_layer(x, offsets, bias, w_uvqk, w_o, b_o, geo: STUGeometry, seed
         t is not None and t.requires_grad for t in (x, w_uvqk, w_o, b_o, bias))
     return SoftmaxSTULayerFunction.apply(x, offsets, bias, w_uvqk, w_o, b_o, geo, int(seed),
                                          seed_offset, grad_on, bool(return_uvqk))
+
+
+# ------------------------------------------------------------------ per-head softmax attention
+
+def _columns(x):
+    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+
+
+class _JaggedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, offsets, causal: bool, scale: float, grad_on: bool):
+        q, k, v = _columns(q), _columns(k), _columns(v)
+        rows, H, d = q.shape
+        Hkv, dv = k.shape[1], v.shape[2]
+        out = torch.empty(rows, H, dv, dtype=q.dtype, device=q.device)
+        lse = torch.empty(H, rows, dtype=torch.float32, device=q.device) if grad_on else None
+        ctx.call = (offsets.numel() - 1, rows, H, Hkv, d, dv, int(causal), scale,
+                    int(q.dtype == torch.bfloat16))
+        with _on(q.device):
+            _lib.call("gr_jagged_attn_fwd", *_strided(q), *_strided(k), *_strided(v),
+                      offsets.data_ptr(), *ctx.call, out.data_ptr(), _lib.ptr(lse), _stream())
+        if grad_on:
+            ctx.save_for_backward(q, k, v, offsets, out, lse)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, offsets, out, lse = ctx.saved_tensors
+        dout = dout.contiguous()
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        n = _lib.lib().gr_jagged_attn_bwd_workspace_size(q.shape[0], q.shape[1])
+        ws = torch.empty(max(n, 4), dtype=torch.uint8, device=q.device)
+        with _on(q.device):
+            _lib.call("gr_jagged_attn_bwd", *_strided(q), *_strided(k), *_strided(v),
+                      offsets.data_ptr(), *ctx.call, out.data_ptr(), lse.data_ptr(),
+                      dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(),
+                      n, _stream())
+        return dq, dk, dv, None, None, None, None
+
+
+def _strided(x):
+    return x.data_ptr(), x.stride(0), x.stride(1)
+
+
+def jagged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
+                     causal: bool = True, scale: Optional[float] = None) -> torch.Tensor:
+    """Softmax attention of each head over the rows of its own sequence, forward and backward
+    (``gr_jagged_attn_fwd`` / ``_bwd``): out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h'])
+    v[j, h'] over the rows j of i's sequence, j <= i where ``causal``.
+
+    q (rows, H, d), k (rows, Hkv, d), v (rows, Hkv, dv): jagged rows, sequence b being rows
+    offsets[b] .. offsets[b + 1] ((B + 1,) integers, ascending, as asynchronous_complete_cumsum
+    gives them; they are not read on the host).  float32 or bfloat16, 1 <= d, dv <= 256, H a
+    multiple of Hkv (query head h reads key head h' = h // (H // Hkv)); rows and heads of any
+    stride, so column slices of one projection are read in place.  ``scale`` > 0, 1 / sqrt(d)
+    by default.  Returns (rows, H, dv) of q's type; rows past offsets[B] are zero, and so are
+    their gradients.  Softmax and sums are fp32; bfloat16 probabilities enter the products
+    rounded to bfloat16.  No atomics: the same bits every run."""
+    _lib.require_gpu(q, k, v, offsets)
+    if q.dtype not in _FLOATS or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("jagged_attention: q, k and v must be float32 or bfloat16, all the same")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError("jagged_attention: q, k and v must be (rows, heads, columns)")
+    rows, H, d = q.shape
+    if k.shape[0] != rows or v.shape[0] != rows or k.shape[2] != d or v.shape[1] != k.shape[1]:
+        raise ValueError(f"jagged_attention: shapes {tuple(q.shape)}, {tuple(k.shape)}, "
+                         f"{tuple(v.shape)} do not belong together")
+    if k.shape[1] < 1 or H < 1 or H % k.shape[1] != 0:
+        raise ValueError(f"jagged_attention: {H} query heads are no multiple of {k.shape[1]} key heads")
+    if not (1 <= d <= 256 and 1 <= v.shape[2] <= 256):
+        raise ValueError(f"jagged_attention: head widths {d}, {v.shape[2]} outside [1, 256]")
+    if offsets.dim() != 1 or offsets.numel() < 1 or offsets.is_floating_point() or offsets.dtype == torch.bool:
+        raise ValueError("jagged_attention: offsets must be (B + 1,) integers")
+    if any(t.device != q.device for t in (k, v, offsets)):
+        raise ValueError("jagged_attention: all tensors must be on one device")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError(f"jagged_attention: scale must be positive and finite (got {scale})")
+    grad_on = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v))
+    return _JaggedAttention.apply(q, k, v, offsets.to(torch.int64).contiguous(), bool(causal), scale, grad_on)
 
 
 # ------------------------------------------------------------------ cached decoding

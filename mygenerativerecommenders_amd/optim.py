@@ -9,18 +9,30 @@ travel in the kernel arguments (up to 48 tensors per launch), as torch's tensor 
 do, so graph capture and fresh gradient tensors each step both work.  The
 per-parameter state (``exp_avg`` / ``exp_avg_sq`` views into the flat buffers, ``step``)
 has torch's names.  Dense fp32 CUDA tensors only; ``amsgrad`` and ``maximize`` raise.
+
+``state_bits=8`` holds both moments in 8 bits (``gr_adamw8_step``): 2.1 bytes of state an
+element instead of 8.  ``exp_avg`` / ``exp_avg_sq`` are then ``torch.float8_e4m3fn`` and
+``exp_avg_scale`` / ``exp_avg_sq_scale`` hold a power of two for each 64 consecutive elements:
+a moment is code times scale.  Codes are rounded at random from a hash of (element, step), so
+equal gradients give equal bits on every replica and in every run.
 """
 from __future__ import annotations
 
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, ops
+
+
+_BLOCK = 64  # elements that share a scale of an 8-bit moment
 
 
 class FlatAdamW(torch.optim.Optimizer):
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
-                 weight_decay: float = 1e-2, amsgrad: bool = False, maximize: bool = False):
+                 weight_decay: float = 1e-2, amsgrad: bool = False, maximize: bool = False,
+                 state_bits: int = 32):
+        if state_bits not in (8, 32):
+            raise ValueError(f"FlatAdamW: state_bits must be 8 or 32 (got {state_bits})")
         if amsgrad or maximize:
             raise NotImplementedError("FlatAdamW: amsgrad / maximize are not supported")
         if not 0.0 <= lr or not 0.0 <= eps or not 0.0 <= weight_decay:
@@ -29,6 +41,7 @@ class FlatAdamW(torch.optim.Optimizer):
             raise ValueError(f"FlatAdamW: invalid betas {betas}")
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
         self._flat: dict = {}
+        self._bits = state_bits
 
     def _group_state(self, gi: int, group: dict) -> dict:
         fs = self._flat.get(gi)
@@ -39,6 +52,8 @@ class FlatAdamW(torch.optim.Optimizer):
         for p in params:
             if p.device != dev or p.dtype != torch.float32 or not p.is_contiguous() or not p.is_cuda:
                 raise TypeError("FlatAdamW: contiguous fp32 CUDA parameters on one device expected")
+        if self._bits == 8:
+            return self._group_state8(gi, params, dev)
         offs = np.zeros(len(params), np.int64)
         o = 0
         for i, p in enumerate(params):
@@ -53,6 +68,70 @@ class FlatAdamW(torch.optim.Optimizer):
                              "exp_avg_sq": v[off:off + p.numel()].view_as(p)}
         fs = self._flat[gi] = {"m": m, "v": v, "step": step, "done": done, "offs": offs}
         return fs
+
+    def _group_state8(self, gi: int, params: list, dev) -> dict:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FlatAdamW: take a step (or load a state) before capturing one, or the "
+                               "captured graph would clear the moments on every replay")
+        offs = np.zeros(len(params), np.int64)
+        o = 0
+        for i, p in enumerate(params):
+            offs[i] = o
+            o += -(-p.numel() // _BLOCK) * _BLOCK  # scales belong to one tensor each
+        fs = {"exp_avg": torch.zeros(o, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn),
+              "exp_avg_scale": torch.zeros(o // _BLOCK, dtype=torch.float32, device=dev),
+              "exp_avg_sq": torch.zeros(o, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn),
+              "exp_avg_sq_scale": torch.zeros(o // _BLOCK, dtype=torch.float32, device=dev),
+              "step": torch.zeros(1, dtype=torch.float32, device=dev)}
+        for p, off in zip(params, offs.tolist()):
+            n = p.numel()
+            blocks = slice(off // _BLOCK, (off + n + _BLOCK - 1) // _BLOCK)
+            self.state[p] = {"step": fs["step"], "exp_avg": fs["exp_avg"][off:off + n].view_as(p),
+                             "exp_avg_scale": fs["exp_avg_scale"][blocks],
+                             "exp_avg_sq": fs["exp_avg_sq"][off:off + n].view_as(p),
+                             "exp_avg_sq_scale": fs["exp_avg_sq_scale"][blocks]}
+        fs["done"] = torch.zeros(1, dtype=torch.int32, device=dev)
+        fs["offs"] = offs
+        self._flat[gi] = fs
+        return fs
+
+    def flat_state(self, group: int = 0) -> dict:
+        """The flat buffers behind a parameter group's per-parameter state, by torch's names
+        (``exp_avg``, ``exp_avg_sq``, ``step``; with ``state_bits=8`` the two scales too).
+        Tensor i's entries start at its offset: sizes rounded up to 4 elements (32 bits) or
+        64 (8 bits), in the order of the group's parameters."""
+        fs = self._group_state(group, self.param_groups[group])
+        if self._bits == 8:
+            return {n: t for n, t in fs.items() if n not in ("done", "offs")}
+        return {"exp_avg": fs["m"], "exp_avg_sq": fs["v"], "step": fs["step"]}
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        """torch's, with the loaded moments copied into the flat buffers that the step reads.
+        A state of the other ``state_bits`` raises ValueError, and so do parameters of one
+        group that have taken different numbers of steps (the group has one counter)."""
+        names = ("exp_avg", "exp_avg_sq") + (("exp_avg_scale", "exp_avg_sq_scale") if self._bits == 8 else ())
+        for st in state_dict["state"].values():
+            if any(n not in st for n in names) or ("exp_avg_scale" in st) != (self._bits == 8):
+                raise ValueError(f"FlatAdamW: the loaded state does not hold {self._bits}-bit moments")
+        super().load_state_dict(state_dict)
+        loaded = {p: self.state[p] for g in self.param_groups for p in g["params"] if self.state.get(p)}
+        self._flat.clear()
+        for gi, group in enumerate(self.param_groups):
+            have = [p for p in group["params"] if p in loaded]
+            if not have:
+                continue
+            steps = {float(loaded[p]["step"]) for p in have}
+            if len(steps) > 1:
+                raise ValueError(f"FlatAdamW: parameters of one group have taken {sorted(steps)} steps")
+            with torch.no_grad():
+                self._group_state(gi, group)["step"].fill_(steps.pop())
+                for p in have:
+                    for n in names:
+                        to, x = self.state[p][n], loaded[p][n]
+                        if to.shape != x.shape:
+                            raise ValueError(f"FlatAdamW: loaded {n} has shape {tuple(x.shape)}, "
+                                             f"expected {tuple(to.shape)}")
+                        to.copy_(x)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -78,9 +157,16 @@ class FlatAdamW(torch.optim.Optimizer):
                     raise TypeError("FlatAdamW: dense contiguous fp32 gradients expected")
                 pp[i], gp[i], ne[i] = p.data_ptr(), g.data_ptr(), p.numel()
             b1, b2 = group["betas"]
-            _lib.call("gr_adamw_step", pp.ctypes.data, gp.ctypes.data, fs["offs"].ctypes.data,
-                      ne.ctypes.data, n, fs["m"].data_ptr(), fs["v"].data_ptr(),
-                      fs["step"].data_ptr(), fs["done"].data_ptr(), float(group["lr"]), float(b1),
-                      float(b2), float(group["eps"]), float(group["weight_decay"]),
-                      _lib.stream_handle())
+            hyper = (float(group["lr"]), float(b1), float(b2), float(group["eps"]),
+                     float(group["weight_decay"]))
+            lists = (pp.ctypes.data, gp.ctypes.data, fs["offs"].ctypes.data, ne.ctypes.data, n)
+            if self._bits == 8:
+                with ops._on(params[0].device):
+                    _lib.call("gr_adamw8_step", *lists, fs["exp_avg"].data_ptr(),
+                              fs["exp_avg_scale"].data_ptr(), fs["exp_avg_sq"].data_ptr(),
+                              fs["exp_avg_sq_scale"].data_ptr(), fs["step"].data_ptr(),
+                              fs["done"].data_ptr(), *hyper, _lib.stream_handle())
+                continue
+            _lib.call("gr_adamw_step", *lists, fs["m"].data_ptr(), fs["v"].data_ptr(),
+                      fs["step"].data_ptr(), fs["done"].data_ptr(), *hyper, _lib.stream_handle())
         return loss

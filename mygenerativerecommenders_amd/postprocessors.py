@@ -3,7 +3,7 @@
 
 ``L2NormEmbeddingPostprocessor`` (postprocessors.py:34-56) runs the
 ``gr_l2_normalize`` kernel forward and backward; ``LayerNormEmbeddingPostprocessor``
-(postprocessors.py:59-80) is not on the path and keeps plain PyTorch.
+(postprocessors.py:59-80) the ``gr_layer_norm`` kernels where they apply.
 """
 from __future__ import annotations
 
@@ -41,7 +41,9 @@ class L2NormEmbeddingPostprocessor(OutputPostprocessorModule):
 
 
 class LayerNormEmbeddingPostprocessor(OutputPostprocessorModule):
-    """Off the hot path (postprocessors.py:59-80): plain PyTorch."""
+    """postprocessors.py:59-80.  float32 and bfloat16 rows on the GPU run ``ops.layer_norm``;
+    everything else (CPU tensors, other types, autocast, traced or transformed calls) is torch's
+    ``F.layer_norm``."""
 
     def __init__(self, embedding_dim: int, eps: float = 1e-6) -> None:
         super().__init__()
@@ -53,5 +55,10 @@ class LayerNormEmbeddingPostprocessor(OutputPostprocessorModule):
 
     def forward(self, output_embeddings: torch.Tensor) -> torch.Tensor:
         output_embeddings = output_embeddings[..., : self._embedding_dim]
+        if (output_embeddings.is_cuda and output_embeddings.dtype in (torch.float32, torch.bfloat16)
+                and output_embeddings.shape[-1] == self._embedding_dim
+                and not torch.is_autocast_enabled() and not torch.compiler.is_compiling()
+                and not torch._C._are_functorch_transforms_active()):
+            return ops.layer_norm(output_embeddings, eps=self._eps)
         return F.layer_norm(output_embeddings, normalized_shape=(self._embedding_dim,),
                             eps=self._eps)

@@ -1,0 +1,310 @@
+"""ops.jagged_attention against the formula in 64 bits, forward and gradients.
+
+Bounds are derived, not fitted.  With u = 2^-24 (half a step of fp32) and b = 2^-8 (half a
+step of bf16; 0 where the operands are fp32):
+  * a score is a sum of d products: error at most (d + 2) u scale sum|q k| =: e, which is the
+    relative error of its probability, as is the log-sum's (the largest e of the row) and that
+    of the exponential and its argument, (2 + |score|) u.  So P is off by at most
+    r P, r = e + max e + (8 + n + 2 max|score|) u, n terms in its sum;
+  * a product with P (rounded to bf16: b P) over n rows is off by (r + b + n u) P|x|;
+  * D = sum(dO O) is off by b dO|O| (O is held in the operands' type) + what O is off by times
+    |dO| + dv u dO|O|, dP by dv u |dO||V|, so dS by r |dS| + P (those two);
+  * the result is rounded once more to its type: b of itself."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+def reference(q, k, v, offsets, causal, scale, dout):
+    """(out, dq, dk, dv) in 64 bits and the bound of each, from the inputs' own values."""
+    b = 2.0 ** -8 if q.dtype == torch.bfloat16 else 0.0
+    q, k, v, dout = (t.detach().double() for t in (q, k, v, dout))
+    H, group, d, w = q.shape[1], q.shape[1] // k.shape[1], q.shape[2], v.shape[2]
+    res = [torch.zeros(t.shape, dtype=torch.float64, device=q.device) for t in (dout, q, k, v)]
+    lim = [torch.zeros_like(t) for t in res]
+    ends = offsets.tolist()
+    for s, e in zip(ends, ends[1:]):
+        n = e - s
+        for h in range(H if n else 0):
+            j = h // group
+            Q, K, V, G = q[s:e, h], k[s:e, j], v[s:e, j], dout[s:e, h]
+            S = scale * (Q @ K.T)
+            live = torch.ones(n, n, dtype=torch.bool, device=q.device)
+            if causal:
+                live = live.tril()
+            err = (d + 2) * U * scale * (Q.abs() @ K.abs().T) * live
+            S = S.masked_fill(~live, -math.inf)
+            P = torch.softmax(S, -1)
+            r = err + err.amax(1, keepdim=True) + (8 + n + 2 * (S.abs() * live).nan_to_num(0, 0, 0).amax(1, keepdim=True)) * U
+            O = P @ V
+            eO = (P * (r + b + n * U)) @ V.abs()
+            dP = G @ V.T
+            D = (G * O).sum(1, keepdim=True)
+            eD = ((b + w * U) * (G * O).abs() + G.abs() * eO).sum(1, keepdim=True)
+            dS = P * (dP - D)
+            eS = r * dS.abs() + P * (eD + w * U * (G.abs() @ V.abs().T)) + (b + n * U) * dS.abs()
+            parts = [(O, eO), (scale * (dS @ K), scale * (eS @ K.abs())), (scale * (dS.T @ Q), scale * (eS.T @ Q.abs())),
+                     (P.T @ G, (P * (r + b + n * U)).T @ G.abs())]
+            for i, (at, (x, ex)) in enumerate(zip((h, h, j, j), parts)):
+                res[i][s:e, at] += x
+                lim[i][s:e, at] += ex
+    return res, [t + (b + 4 * U) * x.abs() + 1e-30 for t, x in zip(lim, res)]
+
+
+def make(lengths, H, Hkv, d, dv, dtype, spare=0, seed=0, spread=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed + sum(lengths) + d)
+    offsets = torch.tensor([0] + list(lengths)).cumsum(0).cuda()
+    rows = int(offsets[-1]) + spare
+    wide = torch.randn(rows, H * d + Hkv * (d + dv), device="cuda", generator=g).to(dtype)
+    q = (spread * wide[:, :H * d]).to(dtype).view(rows, H, d)
+    k = wide[:, H * d:(H + Hkv) * d].view(rows, Hkv, d)
+    v = wide[:, (H + Hkv) * d:].view(rows, Hkv, dv)
+    dout = torch.randn(rows, H, dv, device="cuda", generator=g).to(dtype)
+    return q, k, v, offsets, dout
+
+
+def run(q, k, v, offsets, dout, **kw):
+    from mygenerativerecommenders_amd import ops
+    q, k, v = (t.detach().requires_grad_(True) for t in (q, k, v))
+    out = ops.jagged_attention(q, k, v, offsets, **kw)
+    return [out.detach(), *torch.autograd.grad(out, (q, k, v), dout)]
+
+
+def check(q, k, v, offsets, dout, causal=True, scale=None):
+    got = run(q, k, v, offsets, dout, causal=causal, **({} if scale is None else {"scale": scale}))
+    ref, lim = reference(q, k, v, offsets, causal, q.shape[2] ** -0.5 if scale is None else scale, dout)
+    for name, x, y, e in zip(("out", "dq", "dk", "dv"), got, ref, lim):
+        assert x.dtype == q.dtype and x.shape == y.shape
+        assert torch.isfinite(x).all(), name
+        worst = ((x.double() - y).abs() / e).max().item() if x.numel() else 0.0
+        assert worst <= 1.0, (name, worst)
+    return got
+
+
+DTYPES = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+
+
+@DTYPES
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+@pytest.mark.parametrize("lengths", [[1], [0, 1, 2, 0, 3], [31, 32, 33], [127, 128, 129, 0], [64, 65, 300, 7, 211]],
+                         ids=str)
+def test_lengths(lengths, causal, dtype):
+    check(*make(lengths, 2, 2, 50, 50, dtype), causal=causal)
+
+
+@DTYPES
+@pytest.mark.parametrize("d,dv", [(1, 1), (3, 5), (7, 4), (8, 8), (33, 50), (50, 33), (64, 64), (65, 64), (100, 96),
+                                  (128, 128), (129, 40), (40, 200), (255, 256), (256, 256)])
+def test_widths(d, dv, dtype):
+    check(*make([37, 130, 1], 2, 1, d, dv, dtype))
+
+
+@DTYPES
+@pytest.mark.parametrize("H,Hkv", [(1, 1), (3, 3), (4, 1), (6, 2), (8, 8)])
+def test_shared_heads(H, Hkv, dtype):
+    check(*make([150, 33, 0, 70], H, Hkv, 64, 64, dtype))
+
+
+@DTYPES
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_long_rows(d, dtype):
+    check(*make([1111, 2059], 1, 1, d, d, dtype), causal=d != 128)
+
+
+@DTYPES
+def test_many_short_sequences(dtype):
+    lengths = [(7 * i) % 12 for i in range(700)]
+    check(*make(lengths, 2, 1, 16, 24, dtype))
+
+
+@DTYPES
+@pytest.mark.parametrize("d", [50, 256])
+def test_rows_of_no_sequence_are_zero_and_never_read(d, dtype):
+    q, k, v, offsets, dout = make([40, 0, 129], 2, 1, d, d, dtype, spare=300)
+    n = int(offsets[-1])
+    want = run(q[:n], k[:n], v[:n], offsets, dout[:n])
+    q, k, v, dout = (t.clone() for t in (q, k, v, dout))
+    for t in (q, k, v, dout):
+        t[n:] = float("nan")
+    for x, y in zip(run(q, k, v, offsets, dout), want):
+        assert torch.equal(x[:n], y) and (x[n:] == 0).all()
+
+
+@DTYPES
+def test_neighbours_do_not_leak(dtype):
+    """Infinities and NaN stay in their sequence and key head."""
+    q, k, v, offsets, dout = make([70, 100, 45], 4, 2, 50, 50, dtype)
+    want = run(q, k, v, offsets, dout)
+    k, v = k.clone(), v.clone()
+    k[130, 1] = float("nan")  # row 60 of the second sequence
+    v[131, 1] = float("inf")
+    got = run(q, k, v, offsets, dout)
+    for x, y in zip(got, want):
+        own = x.shape[1] // 2
+        assert torch.equal(x[:70], y[:70]) and torch.equal(x[170:], y[170:])
+        assert torch.equal(x[:, :own], y[:, :own])
+    assert torch.isnan(got[0][130:170, 2:]).all()
+
+
+@DTYPES
+def test_large_scores(dtype):
+    """Scores in the hundreds: a softmax without its running maximum would overflow."""
+    q, k, v, offsets, dout = make([200, 64], 2, 2, 64, 64, dtype, spread=60.0)
+    check(q, k, v, offsets, dout)
+
+
+@DTYPES
+def test_scale(dtype):
+    check(*make([90, 40], 2, 1, 48, 48, dtype), scale=0.03)
+
+
+@DTYPES
+def test_strides_and_offset_types(dtype):
+    q, k, v, offsets, dout = make([77, 130], 4, 2, 40, 40, dtype)
+    want = run(q, k, v, offsets, dout)
+    heads_first = [t.permute(1, 0, 2).contiguous().permute(1, 0, 2) for t in (q, k, v, dout)]
+    odd = [torch.cat([torch.zeros_like(t[..., :1]), t], -1)[..., 1:] for t in (q, k, v)]
+    column = [t.permute(0, 2, 1).contiguous().permute(0, 2, 1) for t in (q, k, v)]
+    for args in ((*heads_first[:3], offsets, heads_first[3]), (*odd, offsets.to(torch.int32), dout),
+                 (*column, offsets, dout)):
+        for x, y in zip(run(*args), want):
+            assert torch.equal(x, y)
+
+
+def test_broadcast_keys_get_summed_gradients():
+    """One row of keys and values expanded over all rows: autograd sums the rows' gradients."""
+    from mygenerativerecommenders_amd import ops
+    q, k, v, offsets, dout = make([50, 20], 2, 1, 32, 32, torch.float32)
+    k1, v1 = (t[:1].detach().clone().requires_grad_(True) for t in (k, v))
+    out = ops.jagged_attention(q, k1.expand_as(k), v1.expand_as(v), offsets)
+    gk, gv = torch.autograd.grad(out, (k1, v1), dout)
+    _, _, dk, dv = run(q, k1.detach().expand_as(k).contiguous(), v1.detach().expand_as(v).contiguous(), offsets, dout)
+    assert torch.allclose(gk, dk.sum(0, keepdim=True), rtol=1e-5, atol=1e-5)
+    assert torch.allclose(gv, dv.sum(0, keepdim=True), rtol=1e-5, atol=1e-5)
+
+
+def test_gradients_against_differences():
+    """Central differences (h = 1e-2) of the sum along random unit directions.  Their own error:
+    h^2 / 6 = 1.7e-5 times a third derivative (of the order of the gradient's norm: scores are
+    of order one), and the forward's fp32 error over 2h, about 1e-6 sqrt(outputs) / 2e-2 = 3e-3
+    of an output's size at most; the gradients' norms are some tens."""
+    from mygenerativerecommenders_amd import ops
+    q, k, v, offsets, dout = make([19, 40], 2, 1, 24, 24, torch.float32)
+    _, *grads = run(q, k, v, offsets, dout)
+    h, gen = 1e-2, torch.Generator(device="cuda").manual_seed(5)
+    for i, g in enumerate(grads):
+        way = torch.randn(g.shape, device="cuda", generator=gen)
+        way /= way.norm()
+        side = []
+        for sign in (1, -1):
+            args = [q, k, v]
+            args[i] = args[i] + sign * h * way
+            side.append((ops.jagged_attention(*args, offsets).double() * dout.double()).sum())
+        diff = ((side[0] - side[1]) / (2 * h)).item()
+        assert abs(diff - (g * way).sum().item()) <= 2e-3 * max(1.0, g.norm().item()), i
+
+
+@DTYPES
+def test_same_bits_every_run_and_on_another_stream(dtype):
+    args = make([300, 211, 128], 4, 2, 64, 64, dtype)
+    want = run(*args)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run(*args)
+    torch.cuda.current_stream().wait_stream(side)
+    for x, y, z in zip(want, got, run(*args)):
+        assert torch.equal(x, y) and torch.equal(x, z)
+
+
+@DTYPES
+def test_captured_and_replayed(dtype):
+    """Two graphs of forward and backward, replayed in turn with eager work between: each
+    replay reads its own inputs' present values."""
+    q, k, v, offsets, dout = make([100, 0, 211], 2, 1, 50, 50, dtype, spare=9)
+    pairs = []
+    for i in range(2):
+        bufs = [t.clone() for t in (q, k, v, dout)]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(*bufs[:3], offsets, bufs[3])
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = run(*bufs[:3], offsets, bufs[3])
+        pairs.append((graph, bufs, outs))
+    for step in range(4):
+        graph, bufs, outs = pairs[step % 2]
+        for b, t in zip(bufs, (q, k, v, dout)):
+            b.copy_(t * (1 + 0.25 * step))
+        graph.replay()
+        want = run(*[b.clone() for b in bufs[:3]], offsets, bufs[3].clone())
+        torch.cuda.synchronize()
+        for x, y in zip(outs, want):
+            assert torch.equal(x, y), step
+
+
+def test_rows_beyond_32_bits():
+    """Rows whose element offsets pass 2^31 in their buffer: 60,000 rows 40,000 apart, cut into
+    short sequences; the last ones give what a small buffer gives."""
+    stride, rows = 40000, 60000
+    q, k, v, offsets, dout = make([64, 200], 1, 1, 32, 32, torch.bfloat16)
+    want = run(q, k, v, offsets, dout)
+    big = torch.empty(rows * stride, dtype=torch.bfloat16, device="cuda").view(rows, stride)
+    views = []
+    for i, t in enumerate((q, k, v)):
+        view = big[:, 64 * i:64 * i + 32].unflatten(1, (1, 32))
+        view[:rows - 264] = 0
+        view[rows - 264:] = t
+        views.append(view)
+    assert views[0].stride(0) == stride
+    cut = torch.arange(0, rows - 264, 128, device="cuda")
+    ends = torch.cat([cut, torch.tensor([rows - 264, rows - 200, rows], device="cuda")])
+    g = torch.zeros(rows, 1, 32, dtype=torch.bfloat16, device="cuda")
+    g[rows - 264:] = dout
+    for x, y in zip(run(*views, ends, g), want):
+        assert torch.equal(x[rows - 264:], y)
+
+
+def test_refusals():
+    from mygenerativerecommenders_amd import _lib, ops
+    q, k, v, offsets, _ = make([10, 5], 4, 2, 16, 16, torch.float32)
+    with pytest.raises(_lib.GrError, match="CPU tensor"):
+        ops.jagged_attention(q.cpu(), k, v, offsets)
+    with pytest.raises(TypeError):
+        ops.jagged_attention(q.half(), k.half(), v.half(), offsets)
+    with pytest.raises(TypeError):
+        ops.jagged_attention(q, k.bfloat16(), v, offsets)
+    for bad in ((q[0], k, v), (q, k[:3], v), (q, k, v[:, :1]), (q[..., :8], k, v), (q[:, :3], k, v), (q[:, :0], k, v)):
+        with pytest.raises(ValueError):
+            ops.jagged_attention(*bad, offsets)
+    wide = torch.zeros(15, 2, 257, device="cuda")
+    with pytest.raises(ValueError, match="widths"):
+        ops.jagged_attention(wide, wide, wide, offsets)
+    for bad in (offsets.float(), offsets[None], offsets[:0]):
+        with pytest.raises(ValueError, match="offsets"):
+            ops.jagged_attention(q, k, v, bad)
+    for bad in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError, match="scale"):
+            ops.jagged_attention(q, k, v, offsets, scale=bad)
+    q.requires_grad_(True)
+    (g,) = torch.autograd.grad(ops.jagged_attention(q, k, v, offsets).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_empty_batches():
+    from mygenerativerecommenders_amd import ops
+    none = torch.zeros(0, 2, 16, device="cuda", requires_grad=True)
+    out = ops.jagged_attention(none, none, none, torch.zeros(3, dtype=torch.int64, device="cuda"))
+    out.sum().backward()
+    assert out.shape == (0, 2, 16) and none.grad.shape == (0, 2, 16)
+    some = torch.randn(9, 2, 16, device="cuda")
+    for offsets in (torch.zeros(1, dtype=torch.int64, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")):
+        assert (ops.jagged_attention(some, some, some, offsets) == 0).all()

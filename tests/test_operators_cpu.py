@@ -1,0 +1,101 @@
+"""What the attention, layer norm and 8-bit AdamW entries refuse, without a GPU: the checks run
+before any HIP call."""
+import ctypes
+
+import pytest
+import torch
+
+from mygenerativerecommenders_amd import _lib, ops
+from mygenerativerecommenders_amd.optim import FlatAdamW
+
+P = 4096  # a pointer that is never followed: each call below is refused
+
+
+def attn(**kw):
+    a = dict(q=P, ld_q=8, hs_q=8, k=P, ld_k=8, hs_k=8, v=P, ld_v=8, hs_v=8, offsets=P, B=1, rows=4, H=2, Hkv=1, d=8, dv=8,
+             causal=1, scale=1.0, bf16=0)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("bad", [dict(q=None), dict(k=None), dict(v=None), dict(offsets=None), dict(B=-1), dict(rows=-1),
+                                 dict(H=0), dict(Hkv=0), dict(H=3, Hkv=2), dict(d=0), dict(d=257), dict(dv=0), dict(dv=300),
+                                 dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
+                                 dict(rows=1 << 31), dict(rows=1 << 30, H=4096, Hkv=4096)], ids=str)
+def test_attention_refuses(bad):
+    with pytest.raises(_lib.GrError, match="gr_jagged_attn_fwd"):
+        _lib.call("gr_jagged_attn_fwd", *attn(**bad), P, None, None)
+    with pytest.raises(_lib.GrError, match="gr_jagged_attn_bwd"):
+        _lib.call("gr_jagged_attn_bwd", *attn(**bad), P, P, P, P, P, P, P, 1 << 40, None)
+
+
+def test_attention_backward_refuses_missing_buffers():
+    for i in range(7):
+        bufs = [P] * 7
+        bufs[i] = None
+        with pytest.raises(_lib.GrError):
+            _lib.call("gr_jagged_attn_bwd", *attn(), *bufs, 1 << 20, None)
+    n = _lib.lib().gr_jagged_attn_bwd_workspace_size(4, 2)
+    assert n == 32
+    with pytest.raises(_lib.GrError, match="workspace"):
+        _lib.call("gr_jagged_attn_bwd", *attn(), *[P] * 7, n - 1, None)
+    with pytest.raises(_lib.GrError):
+        _lib.call("gr_jagged_attn_fwd", *attn(), None, None, None)
+
+
+def test_layer_norm_refuses():
+    ok = dict(x=P, ld_x=8, rows=4, D=8, w=None, b=None, types=0, eps=1e-6, y=P, ld_y=8, stats=None, stream=None)
+    for bad in (dict(x=None), dict(y=None), dict(rows=-1), dict(D=0), dict(types=4), dict(types=-1), dict(ld_x=7),
+                dict(ld_x=-8), dict(ld_y=7), dict(ld_y=0)):
+        with pytest.raises(_lib.GrError, match="gr_layer_norm_fwd"):
+            _lib.call("gr_layer_norm_fwd", *dict(ok, **bad).values())
+    ok = dict(dy=P, ld_dy=8, x=P, ld_x=8, rows=4, D=8, w=None, types=0, stats=P, dx=P, ld_dx=8, dw=None, db=None, ws=None,
+              n=0, stream=None)
+    for bad in (dict(dy=None), dict(x=None), dict(stats=None), dict(rows=-1), dict(D=0), dict(types=4), dict(ld_dy=7),
+                dict(ld_x=7), dict(ld_dx=7), dict(dw=P), dict(db=P), dict(dw=P, ws=P, n=8)):
+        with pytest.raises(_lib.GrError, match="gr_layer_norm_bwd"):
+            _lib.call("gr_layer_norm_bwd", *dict(ok, **bad).values())
+    assert _lib.lib().gr_layer_norm_bwd_workspace_size(4, 8, 0) >= 2 * 8 * 4
+    assert _lib.lib().gr_layer_norm_bwd_workspace_size(0, 8, 0) == 0
+    _lib.call("gr_layer_norm_fwd", None, 8, 0, 8, None, None, 0, 1e-6, None, 8, None, None)
+
+
+def test_adamw8_refuses():
+    u64, i64 = ctypes.c_uint64 * 1, ctypes.c_int64 * 1
+    hyper = (1e-3, 0.9, 0.999, 1e-8, 0.0, None)
+
+    def call(params=P, grads=P, off=0, numel=8, n=1, bufs=(P,) * 6):
+        lists = [ctypes.addressof(a) for a in (pp, gg, oo, nn)] if n else [None] * 4
+        pp[0], gg[0], oo[0], nn[0] = params, grads, off, numel
+        _lib.call("gr_adamw8_step", *lists, n, *bufs, *hyper)
+
+    pp, gg, oo, nn = u64(), u64(), i64(), i64()
+    for bad in (dict(params=0), dict(grads=0), dict(off=-64), dict(off=32), dict(numel=-1), dict(n=-1),
+                *(dict(bufs=(P,) * i + (None,) + (P,) * (5 - i)) for i in range(6)), dict(bufs=(P + 1,) + (P,) * 5)):
+        with pytest.raises(_lib.GrError, match="gr_adamw8_step"):
+            call(**bad)
+    call(n=0, bufs=(None,) * 6)
+    call(numel=0)  # nothing to do
+
+
+def test_python_entries_refuse_cpu_tensors():
+    x = torch.zeros(3, 2, 8)
+    with pytest.raises(_lib.GrError, match="CPU tensor"):
+        ops.jagged_attention(x, x, x, torch.tensor([0, 3]))
+    with pytest.raises(_lib.GrError, match="CPU tensor"):
+        ops.layer_norm(x)
+    p = torch.nn.Parameter(torch.zeros(8))
+    for bits in (0, 4, 16):
+        with pytest.raises(ValueError, match="state_bits"):
+            FlatAdamW([p], state_bits=bits)
+    p.grad = torch.zeros(8)
+    with pytest.raises(TypeError):
+        FlatAdamW([p], state_bits=8).step()
+
+
+def test_layer_norm_postprocessor_on_the_cpu_is_torchs():
+    from mygenerativerecommenders_amd.postprocessors import LayerNormEmbeddingPostprocessor
+    x = torch.randn(5, 7, 64, dtype=torch.float64, requires_grad=True)
+    y = LayerNormEmbeddingPostprocessor(50)(x)
+    assert torch.equal(y, torch.nn.functional.layer_norm(x[..., :50], (50,), eps=1e-6))
+    assert torch.autograd.gradcheck(LayerNormEmbeddingPostprocessor(6), (x[0, :2, :8].detach().requires_grad_(True),))
