@@ -318,10 +318,12 @@ GR_API int gr_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64
  *   out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h']) v[j, h'],  h' = h / (H / Hkv)
  * q (rows, H, d), k (rows, Hkv, d), v (rows, Hkv, dv): bf16 (bf16 != 0) or fp32, element
  * strides ld_* of a row and hs_* of a head, columns contiguous, no alignment beyond the
- * element's; 1 <= d, dv <= 256, H a multiple of Hkv, scale > 0.  out, dout (rows, H, dv), dq
+ * element's; 16 bytes <= d, dv <= 256 elements, H a multiple of Hkv, scale > 0.  out, dout (rows, H, dv), dq
  * (rows, H, d), dk (rows, Hkv, d), dvv (rows, Hkv, dv) are contiguous.  Rows past
  * offsets[B] get zeros; offsets are clamped to [0, rows].  lse (H, rows): log2 of each row's
- * sum of exp(scaled scores), which the backward needs (forward: NULL if there is none).
+ * sum of exp(scaled scores); out_low (bf16 only, as out): what rounding left off out, so that
+ * the backward's sum(dout out) is that of the unrounded rows.  The backward needs both
+ * (forward: NULL if there is none).
  * The backward recomputes the probabilities; dk / dvv sum over the heads that share them.
  * Accumulation and softmax in fp32; no atomics, the same bits every run.  Workspace:
  * gr_jagged_attn_bwd_workspace_size bytes. */
@@ -329,15 +331,15 @@ GR_API int gr_jagged_attn_fwd(const void* q, int64_t ld_q, int64_t hs_q, const v
                               int64_t ld_k, int64_t hs_k, const void* v, int64_t ld_v,
                               int64_t hs_v, const int64_t* offsets, int B, int64_t rows, int H,
                               int Hkv, int d, int dv, int causal, float scale, int bf16,
-                              void* out, float* lse, void* stream);
+                              void* out, void* out_low, float* lse, void* stream);
 GR_API size_t gr_jagged_attn_bwd_workspace_size(int64_t rows, int H);
 GR_API int gr_jagged_attn_bwd(const void* q, int64_t ld_q, int64_t hs_q, const void* k,
                               int64_t ld_k, int64_t hs_k, const void* v, int64_t ld_v,
                               int64_t hs_v, const int64_t* offsets, int B, int64_t rows, int H,
                               int Hkv, int d, int dv, int causal, float scale, int bf16,
-                              const void* out, const float* lse, const void* dout, void* dq,
-                              void* dk, void* dvv, void* workspace, size_t ws_bytes,
-                              void* stream);
+                              const void* out, const void* out_low, const float* lse,
+                              const void* dout, void* dq, void* dk, void* dvv, void* workspace,
+                              size_t ws_bytes, void* stream);
 
 /* ---------------------------------------------------------------- HSTU attention
  * hstu_bucket_map: the relative-time bucket of every causal (query i, key j) pair of

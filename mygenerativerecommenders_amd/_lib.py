@@ -33,6 +33,7 @@ _CTYPES = {
 
 _lock = threading.Lock()
 _lib = None
+_fns: dict = {}
 
 
 def parse_header(path: str = HEADER_PATH):
@@ -94,14 +95,15 @@ def call(name: str, *args):
     varargs, so a caller written against another ABI version would shift every later
     pointer and size silently.
     """
-    L = lib()
-    fn = getattr(L, name)
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(lib(), name)
     if len(args) != len(fn.argtypes):
         raise GrError(f"{name} takes {len(fn.argtypes)} arguments (gr_hstu.h, ABI "
-                      f"{L.gr_version()}), got {len(args)}")
+                      f"{lib().gr_version()}), got {len(args)}")
     rc = fn(*args)
     if rc != 0:
-        msg = L.gr_last_error().decode(errors="replace")
+        msg = lib().gr_last_error().decode(errors="replace")
         raise GrError(f"{name} failed (status {rc}): {msg}")
 
 
@@ -200,8 +202,15 @@ def ptr(t) -> int | None:
 
 
 def stream_handle(device=None) -> int:
-    import torch as _t
-    return _t.cuda.current_stream(device).cuda_stream
+    """The current stream of ``device`` (default: the current device) as a raw handle."""
+    if device is None:
+        return _raw_stream(torch.cuda.current_device())
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _raw_stream(index: int) -> int:
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # absent from CPU-only builds
+    return torch.cuda.current_stream(index).cuda_stream if get is None else get(index)
 
 
 def require_gpu(*tensors):

@@ -29,6 +29,7 @@ struct JaggedAttnArgs {
   float scale;     // of the scores
   float scale_l2;  // scale / ln 2
   void* out;       // (rows, H, dv)
+  void* out_low;   // bf16: what out's rounding left off, or NULL
   float* lse;      // (H, rows): log2 of each row's sum of 2^(scaled score / ln 2), or NULL
   const void* dout;  // (rows, H, dv)
   void* dq;          // (rows, H, d)
@@ -36,7 +37,33 @@ struct JaggedAttnArgs {
   void* dvv;         // (rows, Hkv, dv)
   float* delta;      // (H, rows): sum(dout * out)
   int64_t slots;     // tiles of the rows per head, see jagged_tile
+  int dma;           // rows can go straight to LDS
+  int heads_per_key; // the backward's key pass: `group`, where that is 1 for its grid
+  int sets, sets_k;  // sets of four waves that share a workgroup's tiles (1 or 2), query and key pass
 };
+
+// Work item of a workgroup.  Workgroups i, i + 8, .. land on one XCD: each XCD takes a
+// contiguous eighth of the items, heads of a group next to each other, so that one L2 serves
+// the tiles and heads that read the same keys and values.  Of a causal sequence's tiles the
+// heavy come first; every other round over the XCD's 32 CUs runs backwards, so that a CU that
+// got a heavy tile gets a light one next.
+struct JaggedWork {
+  int hk, g;
+  int64_t slot;
+};
+__device__ __forceinline__ JaggedWork jagged_work(const JaggedAttnArgs& a, unsigned id) {
+  const unsigned n = gridDim.x, per = n / 8, more = n % 8, x = id % 8;
+  unsigned j = id / 8;
+  const unsigned mine = per + (x < more), round = j / 32 * 32;
+  if (j & 32) j = round + (mine - round < 32 ? mine - round : 32) - 1 - (j - round);
+  const unsigned w = x * per + (x < more ? x : more) + j;
+  const unsigned slots = (unsigned)a.slots, group = (unsigned)a.group;
+  JaggedWork k;
+  k.g = (int)(w % group);
+  k.slot = w / group % slots;
+  k.hk = (int)(w / group / slots);
+  return k;
+}
 
 // Tile `slot` of the jagged rows in tiles of BM rows that never cross a sequence: sequence b
 // owns the slots from offsets[b] / BM + b on, which always leaves it enough of them, so
@@ -73,33 +100,24 @@ __device__ __forceinline__ JaggedTile jagged_tile(const int64_t* offsets, int B,
   return t;
 }
 
-// 16 bytes of a row from column c, for rows of `d` elements of any alignment, in two steps so
-// that the first can stay in flight: ja_load16 reads inside the row always (the vector that
-// would cross its end is read up against it), ja_fix16 moves such a vector's elements down
-// and clears what lies past column d, or all of it where `ok` is false.
+// 16 bytes of a row from column c, for rows of `d` >= 16 bytes of any alignment, in two steps
+// so that the first can stay in flight: ja_load16 reads inside the row always (the vector
+// that would cross its end is read up against it), ja_fix16 moves such a vector's elements
+// down and clears what lies past column d, or all of it where `ok` is false.
 template <typename T>
 __device__ __forceinline__ u32x4_t ja_load16(const T* row, int c, int d) {
   constexpr int V = 16 / sizeof(T);
   struct __attribute__((packed, aligned(sizeof(T)))) P {
     u32x4_t v;
   };
-  if (d >= V) return reinterpret_cast<const P*>(row + min(c, d - V))->v;  // uniform
-  T x[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) x[i] = row[min(i, d - 1)];
-  u32x4_t r;
-  __builtin_memcpy(&r, x, 16);
-  return r;
+  return reinterpret_cast<const P*>(row + min(c, d - V))->v;
 }
 template <typename T>
 __device__ __forceinline__ u32x4_t ja_fix16(u32x4_t x, int c, int d, bool ok) {
   constexpr int V = 16 / sizeof(T);
   if (d % V != 0) {  // uniform
     unsigned __int128 w = __builtin_bit_cast(unsigned __int128, x);
-    if (d > V)
-      w >>= max(c + V - d, 0) * 8 * (int)sizeof(T) & 127;  // c >= d is cleared below
-    else
-      w &= ~(unsigned __int128)0 >> (V - d) * 8 * (int)sizeof(T);
+    w >>= max(c + V - d, 0) * 8 * (int)sizeof(T) & 127;  // c >= d is cleared below
     x = __builtin_bit_cast(u32x4_t, w);
   }
 #pragma unroll
@@ -107,34 +125,84 @@ __device__ __forceinline__ u32x4_t ja_fix16(u32x4_t x, int c, int d, bool ok) {
   return x;
 }
 
-// R rows of DP columns of a jagged operand, through the registers into LDS (256 threads).
+// LDS tiles: R rows of DP columns in 16-byte units, 64 of them (RPI rows, 1 KB: what one
+// load-to-LDS instruction writes) followed by one of padding; unit c of row r at place
+// c ^ swizzle(r) of its row.  Read by rows (each lane a row, the same unit) 16 rows cover the 64
+// banks once; read transposed (4 neighbouring units of 8 rows) no bank is hit more often than
+// the bytes take.  Swizzles change few bits, so that most of an address is a constant.
+template <typename T, int DP>
+struct JaTile {
+  static constexpr int V = 16 / sizeof(T), UNITS = DP / V, RPI = 64 / UNITS;
+  static constexpr int BITS = RPI == 8 ? 6 : RPI == 4 ? 12 : RPI == 2 ? 8 : 0;  // that a swizzle changes
+  static __host__ __device__ constexpr int size(int rows) { return rows / RPI * 65; }
+  static __device__ __forceinline__ int swizzle(int r) {
+    return RPI == 8 ? (r >> 1 & 3) << 1 : RPI == 4 ? (r & 3) << 2 : RPI == 2 ? (r & 1) << 3 : 0;
+  }
+  // Unit c0 + cl of row r0 + r: r0 a multiple of 8, c0 of LOW > cl; r0 and c0 constants.
+  template <int LOW>
+  static __device__ __forceinline__ int unit(int r0, int r, int c0, int cl) {
+    const int f = swizzle(r);
+    return r / RPI * 65 + r % RPI * UNITS + (cl ^ (f & (LOW - 1))) + ((c0 & BITS) ^ (f & ~(LOW - 1))) +
+           (c0 & ~BITS) + size(r0);
+  }
+};
+// Brings R rows of a jagged operand into an LDS tile, with a set of four waves.  DMA: straight from
+// memory (buffer_load_dwordx4 to LDS; rows of a multiple of 16 bytes, 16-byte aligned), issued
+// where the compiler does not see it, so that it does not wait for it at the next LDS read:
+// ja_landed() waits and meets the other waves.  The descriptor ends with the sequence's last
+// row, so rows past it come as zeros.  Otherwise through registers.
+template <typename T, int DP, int R, bool DMA>
+struct JaStage;
 template <typename T, int DP, int R>
-struct JaStage {
-  static constexpr int V = 16 / sizeof(T), CPR = DP / V, PER = R * CPR / 256;
-  static_assert(R * CPR % 256 == 0, "whole passes");
-  u32x4_t x[PER];
-  __device__ __forceinline__ void load(const T* base, int64_t ld, int r0, int len, int d) {
+struct JaStage<T, DP, R, true> {
+  using Tile = JaTile<T, DP>;
+  static constexpr int N = R * Tile::UNITS / 256;  // instructions of a wave
+  static_assert(R * Tile::UNITS % 256 == 0 && Tile::UNITS <= 64, "whole instructions");
+  __device__ __forceinline__ void load(const T* base, int64_t ld, int r0, int len, int d, u32x4_t* tile) {
+    constexpr int SZ = sizeof(T);
+    const int lane = threadIdx.x & 63, r = (wave_id() & 3) * Tile::RPI + lane / Tile::UNITS;
+    const int c = (lane % Tile::UNITS ^ Tile::swizzle(r)) * Tile::V;
+    const uint32_t at = __builtin_amdgcn_readfirstlane(
+        (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u32x4_t*)tile + 1040u * (wave_id() & 3));
+    const uint64_t p = (uint64_t)(base + (int64_t)r0 * ld);
+    const int64_t bytes = ((int64_t)(len - r0 - 1) * ld + d) * SZ;
+    const u32x4_t desc = {(uint32_t)p, (uint32_t)(p >> 32) & 0xFFFFu, (uint32_t)(bytes < 0x7FFFFFFF ? bytes : 0x7FFFFFFF),
+                          0x00020000u};
+    const uint32_t off = c < d ? (uint32_t)(r * (int)ld + c) * SZ : (uint32_t)OOB_OFF;  // ld < 2^22
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int at = threadIdx.x + 256 * i;
-      x[i] = ja_load16<T>(base + (int64_t)min(r0 + at / CPR, len - 1) * ld, at % CPR * V, d);
+    for (int i = 0; i < N; ++i) {
+      uint32_t keep;
+      asm volatile(
+          "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
+          : "=&s"(keep)
+          : "s"(at + 4160u * i), "v"(off), "s"(desc), "s"(4 * Tile::RPI * SZ * i * (int)ld)
+          : "memory");
     }
   }
-  __device__ __forceinline__ void store(T* lds, int stride, int r0, int len, int d) {
-    if (r0 + R > len || d != DP) {  // uniform
+  __device__ __forceinline__ void store(u32x4_t*, int, int, int) {}
+};
+template <typename T, int DP, int R>
+struct JaStage<T, DP, R, false> {
+  using Tile = JaTile<T, DP>;
+  static constexpr int N = R * Tile::UNITS / 256;
+  static_assert(R * Tile::UNITS % 256 == 0, "whole passes");
+  u32x4_t x[N];
+  __device__ __forceinline__ void load(const T* base, int64_t ld, int r0, int len, int d, u32x4_t*) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int at = threadIdx.x + 256 * i;
-        x[i] = ja_fix16<T>(x[i], at % CPR * V, d, r0 + at / CPR < len);
-      }
+    for (int i = 0; i < N; ++i) {
+      const int at = (threadIdx.x & 255) + 256 * i;
+      x[i] = ja_load16<T>(base + (int64_t)min(r0 + at / Tile::UNITS, len - 1) * ld, at % Tile::UNITS * Tile::V, d);
     }
+  }
+  __device__ __forceinline__ void store(u32x4_t* tile, int r0, int len, int d) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int at = threadIdx.x + 256 * i;
-      *reinterpret_cast<u32x4_t*>(lds + at / CPR * stride + at % CPR * V) = x[i];
+    for (int i = 0; i < N; ++i) {
+      const int at = (threadIdx.x & 255) + 256 * i, r = at / Tile::UNITS, c = at % Tile::UNITS;
+      tile[r / Tile::RPI * 65 + r % Tile::RPI * Tile::UNITS + (c ^ Tile::swizzle(r))] = ja_fix16<T>(x[i], c * Tile::V, d, r0 + r < len);
     }
   }
 };
+__device__ __forceinline__ void ja_landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Operand fragments.  `K` contraction steps of a fragment: 16 (bf16) or 8 (fp32); lane half
 // h holds the 16 bytes of columns K s + (K / 2) h on of row lane % 32.
@@ -144,9 +212,9 @@ template <>
 struct JaFrag<__bf16> {
   static constexpr int K = 16;
   static __device__ __forceinline__ f32x16 mma(u32x4_t a, u32x4_t b, f32x16 c) { return mfma32(a, b, c); }
-  // A product that contracts 32 rows held in accumulators `p`: c += X^T p with X the LDS
-  // rows of a tile, columns c0 .. c0 + 31.  `p` is rounded to bf16 (half a step: 2^-9 of each
-  // probability, as its bf16 neighbours in the product).
+  // A product that contracts 32 rows held in accumulators `p`: c += X^T p with X rows r0 ..
+  // r0 + 31 of a tile, columns 32 t .. 32 t + 31.  `p` is rounded to bf16 (half a step: 2^-8 of
+  // each value), as its neighbours in the product are bf16.
   struct Rows {
     u32x4_t x[2];
     __device__ __forceinline__ explicit Rows(const f32x16& p) {
@@ -155,10 +223,20 @@ struct JaFrag<__bf16> {
         x[s] = u32x4_t{pack_bf16(p[8 * s], p[8 * s + 1]), pack_bf16(p[8 * s + 2], p[8 * s + 3]),
                        pack_bf16(p[8 * s + 4], p[8 * s + 5]), pack_bf16(p[8 * s + 6], p[8 * s + 7])};
     }
-    __device__ __forceinline__ f32x16 mma(const __bf16* tile, int stride, int c0, f32x16 c) const {
-      const int lane = threadIdx.x & 63;
+    // Transposed reads: lane 4 q + p of a 16-lane group addresses row q, columns 4 p on of a
+    // 4 x 16 block and receives column lane % 16 of its 4 rows.
+    template <int DP>
+    __device__ __forceinline__ f32x16 mma(const u32x4_t* tile, int r0, int t, f32x16 c) const {
+      using Tile = JaTile<__bf16, DP>;
+      const int lane = threadIdx.x & 63, g = lane >> 4, q = (lane & 15) >> 2, p = lane & 3;
+      const int row = 4 * (lane >> 5) + q, cl = 2 * (g & 1) + (p >> 1);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) c = mfma32(trB_acc(tile, stride, s, c0, lane), x[s], c);
+      for (int s = 0; s < 2; ++s) {
+        const u32x4_t *lo = tile + Tile::template unit<4>(r0 + 16 * s, row, 4 * t, cl), *hi = lo + Tile::size(8);
+        const u32x2_t a = tr16(reinterpret_cast<const __bf16*>(lo) + 4 * (p & 1)),
+                      b = tr16(reinterpret_cast<const __bf16*>(hi) + 4 * (p & 1));
+        c = mfma32(u32x4_t{a.x, a.y, b.x, b.y}, x[s], c);
+      }
       return c;
     }
   };
@@ -177,11 +255,16 @@ struct JaFrag<float> {
   struct Rows {
     const f32x16& x;
     __device__ __forceinline__ explicit Rows(const f32x16& p) : x(p) {}
-    __device__ __forceinline__ f32x16 mma(const float* tile, int stride, int c0, f32x16 c) const {
+    template <int DP>
+    __device__ __forceinline__ f32x16 mma(const u32x4_t* tile, int r0, int t, f32x16 c) const {
+      using Tile = JaTile<float, DP>;
       const int lane = threadIdx.x & 63, h = lane >> 5;
-      const float* at = tile + 4 * h * stride + c0 + (lane & 31);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) c = mma1(at[((r & 3) + 8 * (r >> 2)) * stride], x[r], c);
+      for (int r = 0; r < 16; ++r) {
+        const float* at = reinterpret_cast<const float*>(
+            tile + Tile::size(4) * h + Tile::template unit<8>(r0 + 8 * (r >> 2), r & 3, 8 * t, (lane & 31) / 4));
+        c = mma1(at[lane & 3], x[r], c);
+      }
       return c;
     }
   };
@@ -219,24 +302,33 @@ struct JaRows {
   }
 };
 
-// c = X Y^T over 32 x 32: X rows from LDS (row-major tile), Y the wave's fragments.
+// c = X Y^T over 32 x 32: X rows r0 .. r0 + 31 of an LDS tile, Y the wave's fragments.
 template <typename T, int DP, bool KEEP>
-__device__ __forceinline__ f32x16 ja_scores(const T* tile, int stride, JaRows<T, DP, KEEP>& y) {
+__device__ __forceinline__ f32x16 ja_scores(const u32x4_t* tile, int r0, JaRows<T, DP, KEEP>& y) {
   using F = JaFrag<T>;
+  using Tile = JaTile<T, DP>;
   const int lane = threadIdx.x & 63;
-  const T* row = tile + (lane & 31) * stride + F::K / 2 * (lane >> 5);
   f32x16 c = f16_zero();
 #pragma unroll
   for (int s = 0; s < DP / F::K; ++s) {
-    if (s % 8 == 0) y.renew();
-    c = F::mma(*reinterpret_cast<const u32x4_t*>(row + F::K * s), y.at(s), c);
+    if (s % 4 == 0) y.renew();
+    c = F::mma(tile[Tile::template unit<2>(r0, lane & 31, 2 * s, lane >> 5)], y.at(s), c);
   }
   return c;
 }
 
+template <typename T>
+__device__ __forceinline__ void ja_floats(u32x4_t x, float (&o)[16 / sizeof(T)]) {
+  T t[16 / sizeof(T)];
+  __builtin_memcpy(t, &x, 16);
+#pragma unroll
+  for (int i = 0; i < 16 / (int)sizeof(T); ++i) o[i] = (float)t[i];
+}
+
 // Accumulators of a transposed result (register = column of the row lane % 32) to memory.
 template <typename T>
-__device__ __forceinline__ void ja_store_t(T* row, int c0, int width, const f32x16& v, float f, bool ok) {
+__device__ __forceinline__ void ja_store_t(T* row, int c0, int width, const f32x16& v, float f, bool ok,
+                                           T* low = nullptr) {
   const int h = (threadIdx.x & 63) >> 5;
   if (!ok) return;
 #pragma unroll
@@ -250,10 +342,19 @@ __device__ __forceinline__ void ja_store_t(T* row, int c0, int width, const f32x
 #pragma unroll
       for (int i = 0; i < 4; ++i) p.v[i] = (T)(v[4 * g + i] * f);
       *reinterpret_cast<P*>(row + c) = p;
+      if (low) {  // what the rounding left off
+        P e;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e.v[i] = (T)(v[4 * g + i] * f - (float)p.v[i]);
+        *reinterpret_cast<P*>(low + c) = e;
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (c + i < width) row[c + i] = (T)(v[4 * g + i] * f);
+        if (c + i < width) {
+          row[c + i] = (T)(v[4 * g + i] * f);
+          if (low) low[c + i] = (T)(v[4 * g + i] * f - (float)row[c + i]);
+        }
     }
   }
 }
@@ -261,23 +362,46 @@ __device__ __forceinline__ void ja_store_t(T* row, int c0, int width, const f32x
 // Zeros in `width` columns of n rows.
 template <typename T>
 __device__ __forceinline__ void ja_zero(T* base, int64_t ld, int n, int width) {
-  for (int i = threadIdx.x; i < n * width; i += 256) base[(int64_t)(i / width) * ld + i % width] = (T)0.f;
+  for (int i = threadIdx.x; i < n * width; i += blockDim.x) base[(int64_t)(i / width) * ld + i % width] = (T)0.f;
 }
 
-__device__ __forceinline__ float swap_half(float v) { return __shfl_xor(v, 32, 64); }
+// Two sets of waves that each took every other tile join their sums: the second set's
+// accumulators pass through LDS (4 KB a tile and wave; the tiles' own space).
+template <int DT>
+__device__ __forceinline__ void ja_give(float* lds, const f32x16 (&v)[DT]) {
+  float* at = lds + ((wave_id() & 3) * DT * 16) * 64 + (threadIdx.x & 63);
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) at[(i * 16 + r) * 64] = v[i][r];
+}
+template <int DT>
+__device__ __forceinline__ void ja_take(const float* lds, f32x16 (&v)[DT], float mine = 1.f, float its = 1.f) {
+  const float* at = lds + ((wave_id() & 3) * DT * 16) * 64 + (threadIdx.x & 63);
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      if (r % 8 == 0) __builtin_amdgcn_sched_barrier(0);  // few of the reads at a time: registers
+      v[i][r] = v[i][r] * mine + at[(i * 16 + r) * 64] * its;
+    }
+}
 
-// LDS row strides (elements).  Read by rows (16 bytes a lane) a stride of an odd number of
-// 16-byte units spreads the banks; read transposed, 4 or 8 rows at once, one of 64 bytes
-// beyond a multiple of 128 does.
-template <typename T>
-__host__ __device__ constexpr int ja_row_stride(int dp) { return dp + 16 / (int)sizeof(T); }
-template <typename T>
-__host__ __device__ constexpr int ja_col_stride(int dp) { return dp + (sizeof(T) == 2 ? 32 : 8); }
+// Maximum and sum over a lane and its counterpart in the other half of the wave.
+__device__ __forceinline__ float half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
 // Whether a wave's 32 rows of an operand (and the accumulators beside them) fit its registers.
 template <typename T, int DP>
 constexpr bool ja_keep = sizeof(T) == 2 || DP <= 128;
 
-int jagged_attn_check(const char* what, const JaggedAttnArgs& a, int H);
+// Checks the sizes and fills in the rest of the arguments.
+int jagged_attn_check(const char* what, JaggedAttnArgs& a, int H, int bf16);
 
 }  // namespace gr

@@ -16,19 +16,16 @@
 namespace gr {
 
 // dQ: one workgroup per 128 query rows and head, a wave per 32 rows, tiles of BN keys.
-template <typename T, int DP, int BN>
-__global__ __launch_bounds__(256) void jagged_attn_dq_kernel(JaggedAttnArgs a) {
+template <typename T, int DP, int BN, bool DMA, int SETS>
+__global__ __launch_bounds__(256 * SETS) void jagged_attn_dq_kernel(JaggedAttnArgs a) {
   using F = JaFrag<T>;
-  constexpr int BM = 128, NB = BN / 32, DT = DP / 32;
-  constexpr int SK = ja_col_stride<T>(DP), SV = ja_row_stride<T>(DP);
-  __shared__ __attribute__((aligned(16))) T lk[BN * SK];
-  __shared__ __attribute__((aligned(16))) T lv[BN * SV];
-  const int64_t w = blockIdx.x;
-  const int g = (int)(w % a.group);
-  const int64_t ws = w / a.group;
-  const int hk = (int)(ws / a.slots), head = hk * a.group + g;
-  const int H = a.Hkv * a.group;
-  const JaggedTile t = jagged_tile<BM>(a.offsets, a.B, a.rows, a.slots - 1 - ws % a.slots);
+  using Tile = JaTile<T, DP>;
+  constexpr int BM = 128, NB = BN / 32, DT = DP / 32, TILE = Tile::size(BN);
+  __shared__ u32x4_t lds[SETS * 4 * TILE];
+  static_assert(SETS == 1 || sizeof(lds) >= 4 * DT * 16 * 256, "a set's sums fit");
+  const JaggedWork wk = jagged_work(a, blockIdx.x);
+  const int head = wk.hk * a.group + wk.g, H = a.Hkv * a.group;
+  const JaggedTile t = jagged_tile<BM>(a.offsets, a.B, a.rows, a.slots - 1 - wk.slot);
   if (t.len == 0) return;
   T* dq = (T*)a.dq + ((t.s0 + t.r0) * H + head) * a.d;
   if (t.tail) {
@@ -36,65 +33,86 @@ __global__ __launch_bounds__(256) void jagged_attn_dq_kernel(JaggedAttnArgs a) {
     return;
   }
   const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5;
-  const int q0 = t.r0 + 32 * wave, qi = q0 + (lane & 31);
+  const int set = SETS > 1 ? wave >> 2 : 0;  // takes tiles set, set + SETS, ..
+  u32x4_t *lk = lds + set * 4 * TILE, *lv = lk + 2 * TILE;
+  const int q0 = t.r0 + 32 * (wave & 3), qi = q0 + (lane & 31);
   const bool ok = qi < t.len;
-  const T* kb = (const T*)a.k + t.s0 * a.ld_k + hk * a.hs_k;
-  const T* vb = (const T*)a.v + t.s0 * a.ld_v + hk * a.hs_v;
+  const T* kb = (const T*)a.k + t.s0 * a.ld_k + wk.hk * a.hs_k;
+  const T* vb = (const T*)a.v + t.s0 * a.ld_v + wk.hk * a.hs_v;
   const int keys = a.causal ? min(t.len, t.r0 + BM) : t.len;
-  JaStage<T, DP, BN> sk, sv;
-  sk.load(kb, a.ld_k, 0, t.len, a.d);
-  sv.load(vb, a.ld_v, 0, t.len, a.dv);
+  JaStage<T, DP, BN, DMA> sk, sv;
+  const int first = set * BN, step = SETS * BN;
+  if (first < keys) {
+    sk.load(kb, a.ld_k, first, t.len, a.d, lk);
+    sv.load(vb, a.ld_v, first, t.len, a.dv, lv);
+  }
   JaRows<T, DP, ja_keep<T, DP>> q, go;
   q.init((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, a.ld_q, q0, t.len, a.d);
   const int64_t out0 = (t.s0 * H + head) * a.dv;
   go.init((const T*)a.dout + out0, (int64_t)H * a.dv, q0, t.len, a.dv);
   float delta = 0.f;
   {
-    JaRows<T, DP, false> out;
+    JaRows<T, DP, false> out, low;
     out.init((const T*)a.out + out0, (int64_t)H * a.dv, q0, t.len, a.dv);
+    low.init((const T*)(sizeof(T) == 2 ? a.out_low : a.out) + out0, (int64_t)H * a.dv, q0, t.len, a.dv);
 #pragma unroll
     for (int s = 0; s < DP / F::K; ++s) {
-      const u32x4_t x = out.at(s), y = go.at(s);
-      T xs[16 / sizeof(T)], ys[16 / sizeof(T)];
-      __builtin_memcpy(xs, &x, 16);
-      __builtin_memcpy(ys, &y, 16);
+      float x[16 / sizeof(T)], y[16 / sizeof(T)], z[16 / sizeof(T)];
+      ja_floats<T>(out.at(s), x);
+      ja_floats<T>(go.at(s), y);
+      if (sizeof(T) == 2) ja_floats<T>(low.at(s), z);
 #pragma unroll
-      for (int i = 0; i < 16 / (int)sizeof(T); ++i) delta += (float)xs[i] * (float)ys[i];
+      for (int i = 0; i < 16 / (int)sizeof(T); ++i) delta += (sizeof(T) == 2 ? x[i] + z[i] : x[i]) * y[i];
     }
-    delta += swap_half(delta);
+    delta = half_sum(delta);
   }
   const int64_t at = head * a.rows + t.s0 + (ok ? qi : 0);
-  if (ok && half == 0) a.delta[at] = delta;
+  if (ok && half == 0 && set == 0) a.delta[at] = delta;
   const float lse = ok ? a.lse[at] : INFINITY;
   f32x16 acc[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) acc[i] = f16_zero();
-  for (int k0 = 0; k0 < keys; k0 += BN) {
-    __syncthreads();
-    sk.store(lk, SK, k0, t.len, a.d);
-    sv.store(lv, SV, k0, t.len, a.dv);
-    __syncthreads();
-    if (k0 + BN < keys) {
-      sk.load(kb, a.ld_k, k0 + BN, t.len, a.d);
-      sv.load(vb, a.ld_v, k0 + BN, t.len, a.dv);
+  if (first < keys) {
+    sk.store(lk, first, t.len, a.d);
+    sv.store(lv, first, t.len, a.dv);
+  }
+  ja_landed();
+  for (int k0 = first, buf = 0; k0 - first < keys; k0 += step, buf = TILE - buf) {
+    const bool more = k0 + step < keys;
+    if (more) {
+      sk.load(kb, a.ld_k, k0 + step, t.len, a.d, lk + (TILE - buf));
+      sv.load(vb, a.ld_v, k0 + step, t.len, a.dv, lv + (TILE - buf));
     }
-    if (q0 >= t.len || (a.causal && k0 > q0 + 31)) continue;
-    const bool edge = k0 + BN > t.len || (a.causal && k0 + BN - 1 > q0);
-    const int last = a.causal ? min(t.len - 1, qi) : t.len - 1;
+    if (q0 < t.len && k0 < keys && !(a.causal && k0 > q0 + 31)) {
+      const bool edge = k0 + BN > t.len || (a.causal && k0 + BN - 1 > q0);
+      const int last = a.causal ? min(t.len - 1, qi) : t.len - 1;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      f32x16 p = ja_scores(lk + 32 * b * SK, SK, q);
-      const f32x16 dp = ja_scores(lv + 32 * b * SV, SV, go);
+      for (int b = 0; b < NB; ++b) {
+        f32x16 p = ja_scores(lk + buf, 32 * b, q);
+        const f32x16 dp = ja_scores(lv + buf, 32 * b, go);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], a.scale_l2, -lse));
-        if (edge && k0 + 32 * b + (r & 3) + 8 * (r >> 2) + 4 * half > last) p[r] = 0.f;
-        p[r] *= dp[r] - delta;
+        for (int r = 0; r < 16; ++r) {
+          p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], a.scale_l2, -lse));
+          if (edge && k0 + 32 * b + (r & 3) + 8 * (r >> 2) + 4 * half > last) p[r] = 0.f;
+          p[r] *= dp[r] - delta;
+        }
+        const typename F::Rows ds(p);
+#pragma unroll
+        for (int i = 0; i < DT; ++i) acc[i] = ds.template mma<DP>(lk + buf, 32 * b, i, acc[i]);
       }
-      const typename F::Rows ds(p);
-#pragma unroll
-      for (int i = 0; i < DT; ++i) acc[i] = ds.mma(lk + 32 * b * SK, SK, 32 * i, acc[i]);
     }
+    if (more) {
+      sk.store(lk + (TILE - buf), k0 + step, t.len, a.d);
+      sv.store(lv + (TILE - buf), k0 + step, t.len, a.dv);
+    }
+    ja_landed();
+  }
+  if constexpr (SETS > 1) {
+    float* sums = reinterpret_cast<float*>(lds);
+    if (set) ja_give(sums, acc);
+    __syncthreads();
+    if (set) return;
+    ja_take(sums, acc);
   }
   T* row = dq + (int64_t)(ok ? qi - t.r0 : 0) * H * a.d;
 #pragma unroll
@@ -103,19 +121,19 @@ __global__ __launch_bounds__(256) void jagged_attn_dq_kernel(JaggedAttnArgs a) {
 
 // dK, dV: one workgroup per 128 key rows and key head, a wave per 32 keys, tiles of BQ query
 // rows of each query head of the group in turn.  WANT: 1 = dV, 2 = dK, 3 = both in one launch;
-// heads wider than 128 take a launch for each, as both results' accumulators and the keys'
-// fragments do not fit the registers together.
-template <typename T, int DP, int BQ, int WANT>
-__global__ __launch_bounds__(256) void jagged_attn_dkv_kernel(JaggedAttnArgs a) {
+// heads wider than 128 take a launch for each, as both results' accumulators and the
+// keys' fragments do not fit the registers together.
+template <typename T, int DP, int BQ, int WANT, bool DMA, int SETS>
+__global__ __launch_bounds__(256 * SETS) void jagged_attn_dkv_kernel(JaggedAttnArgs a) {
   using F = JaFrag<T>;
-  constexpr int BM = 128, NB = BQ / 32, DT = DP / 32;
-  constexpr int S = ja_col_stride<T>(DP);
-  __shared__ __attribute__((aligned(16))) T lq[BQ * S];
-  __shared__ __attribute__((aligned(16))) T lg[BQ * S];
-  __shared__ __attribute__((aligned(16))) float ll[BQ], ld[BQ];
-  const int64_t w = blockIdx.x;
-  const int hk = (int)(w / a.slots), H = a.Hkv * a.group;
-  const JaggedTile t = jagged_tile<BM>(a.offsets, a.B, a.rows, w % a.slots);
+  using Tile = JaTile<T, DP>;
+  constexpr int BM = 128, NB = BQ / 32, DT = DP / 32, TILE = Tile::size(BQ);
+  __shared__ u32x4_t lds[SETS * 4 * TILE];
+  __shared__ __attribute__((aligned(16))) float lsum[SETS * 4 * BQ];
+  static_assert(SETS == 1 || sizeof(lds) >= 4 * DT * 16 * 256, "a set's sums fit");
+  const JaggedWork wk = jagged_work(a, blockIdx.x);  // group 1: an item per key head
+  const int hk = wk.hk, group = a.heads_per_key, H = a.Hkv * group;
+  const JaggedTile t = jagged_tile<BM>(a.offsets, a.B, a.rows, wk.slot);
   if (t.len == 0) return;
   T* dk = (T*)a.dk + ((t.s0 + t.r0) * a.Hkv + hk) * a.d;
   T* dv = (T*)a.dvv + ((t.s0 + t.r0) * a.Hkv + hk) * a.dv;
@@ -125,8 +143,41 @@ __global__ __launch_bounds__(256) void jagged_attn_dkv_kernel(JaggedAttnArgs a) 
     return;
   }
   const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5;
-  const int k0 = t.r0 + 32 * wave, ki = k0 + (lane & 31);
+  const int set = SETS > 1 ? wave >> 2 : 0, tid = threadIdx.x & 255;
+  u32x4_t *lq = lds + set * 4 * TILE, *lg = lq + 2 * TILE;
+  float *ll = lsum + set * 4 * BQ, *ld = ll + 2 * BQ;
+  const int k0 = t.r0 + 32 * (wave & 3), ki = k0 + (lane & 31);
   const bool ok = ki < t.len;
+  const int first = a.causal ? t.r0 : 0, per = (t.len - first + BQ - 1) / BQ, n = per * group;
+  JaStage<T, DP, BQ, DMA> sq, sg;
+  float rl = 0.f, rd = 0.f;
+  int r0 = first, head = hk * group;  // the tile last loaded: query rows r0 on of a head
+  auto next = [&]() {
+    r0 += BQ;
+    if (r0 >= t.len) {
+      r0 = first;
+      ++head;
+    }
+  };
+  if (set) next();  // a set takes every other tile
+  auto load = [&](int buf) {
+    sq.load((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, a.ld_q, r0, t.len, a.d, lq + buf * TILE);
+    sg.load((const T*)a.dout + (t.s0 * H + head) * a.dv, (int64_t)H * a.dv, r0, t.len, a.dv, lg + buf * TILE);
+    if (tid < BQ) {
+      const int r = r0 + tid;
+      rl = r < t.len ? a.lse[head * a.rows + t.s0 + r] : INFINITY;  // no probability
+      rd = r < t.len ? a.delta[head * a.rows + t.s0 + r] : 0.f;
+    }
+  };
+  auto store = [&](int buf) {
+    sq.store(lq + buf * TILE, r0, t.len, a.d);
+    sg.store(lg + buf * TILE, r0, t.len, a.dv);
+    if (tid < BQ) {
+      ll[buf * BQ + tid] = rl;
+      ld[buf * BQ + tid] = rd;
+    }
+  };
+  if (set < n) load(0);
   JaRows<T, DP, ja_keep<T, DP>> k, v;
   k.init((const T*)a.k + t.s0 * a.ld_k + hk * a.hs_k, a.ld_k, k0, t.len, a.d);
   if (WANT & 2) v.init((const T*)a.v + t.s0 * a.ld_v + hk * a.hs_v, a.ld_v, k0, t.len, a.dv);
@@ -136,63 +187,64 @@ __global__ __launch_bounds__(256) void jagged_attn_dkv_kernel(JaggedAttnArgs a) 
     if (WANT & 2) ak[i] = f16_zero();
     if (WANT & 1) av[i] = f16_zero();
   }
-  const int first = a.causal ? t.r0 : 0, per = (t.len - first + BQ - 1) / BQ, n = per * a.group;
-  JaStage<T, DP, BQ> sq, sg;
-  float rl = 0.f, rd = 0.f;
-  // tile i: query rows first + BQ (i % per) on of head hk * group + i / per
-  auto load = [&](int i) {
-    const int head = hk * a.group + i / per, r0 = first + BQ * (i % per);
-    sq.load((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, a.ld_q, r0, t.len, a.d);
-    sg.load((const T*)a.dout + (t.s0 * H + head) * a.dv, (int64_t)H * a.dv, r0, t.len, a.dv);
-    if (threadIdx.x < BQ) {
-      const int r = r0 + threadIdx.x;
-      rl = r < t.len ? a.lse[head * a.rows + t.s0 + r] : INFINITY;  // no probability
-      rd = r < t.len ? a.delta[head * a.rows + t.s0 + r] : 0.f;
+  if (set < n) store(0);
+  ja_landed();
+  for (int i = set, buf = 0; i - set < n; i += SETS, buf ^= 1) {
+    const int now = r0;
+    if (i + SETS < n) {
+      next();
+      if (SETS > 1) next();
+      load(buf ^ 1);
     }
-  };
-  load(0);
-  for (int i = 0; i < n; ++i) {
-    const int r0 = first + BQ * (i % per);
-    __syncthreads();
-    sq.store(lq, S, r0, t.len, a.d);
-    sg.store(lg, S, r0, t.len, a.dv);
-    if (threadIdx.x < BQ) {
-      ll[threadIdx.x] = rl;
-      ld[threadIdx.x] = rd;
-    }
-    __syncthreads();
-    if (i + 1 < n) load(i + 1);
-    if (k0 >= t.len || (a.causal && r0 + BQ - 1 < k0)) continue;
+    if (k0 < t.len && i < n && !(a.causal && now + BQ - 1 < k0)) {
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int rb = r0 + 32 * b;
-      if (rb >= t.len || (a.causal && rb + 31 < k0)) continue;  // wave-uniform
-      f32x16 p = ja_scores(lq + 32 * b * S, S, k), ds;
-      if (WANT & 2) ds = ja_scores(lg + 32 * b * S, S, v);
-      const bool edge = a.causal && rb < k0 + 31;
+      for (int b = 0; b < NB; ++b) {
+        const int rb = now + 32 * b;
+        if (rb >= t.len || (a.causal && rb + 31 < k0)) continue;  // wave-uniform
+        f32x16 p = ja_scores(lq + buf * TILE, 32 * b, k), ds;
+        if (WANT & 2) ds = ja_scores(lg + buf * TILE, 32 * b, v);
+        const bool edge = a.causal && rb < k0 + 31;
 #pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        const int rr = 32 * b + 8 * r4 + 4 * half;
-        const f4 l4 = *reinterpret_cast<const f4*>(ll + rr), d4 = *reinterpret_cast<const f4*>(ld + rr);
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int rr = 32 * b + 8 * r4 + 4 * half;
+          const f4 l4 = *reinterpret_cast<const f4*>(ll + buf * BQ + rr), d4 = *reinterpret_cast<const f4*>(ld + buf * BQ + rr);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * r4 + e;
-          p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], a.scale_l2, -l4[e]));
-          if (edge && r0 + rr + e < ki) p[r] = 0.f;
-          if (WANT & 2) ds[r] = p[r] * (ds[r] - d4[e]);
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * r4 + e;
+            p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], a.scale_l2, -l4[e]));
+            if (edge && now + rr + e < ki) p[r] = 0.f;
+            if (WANT & 2) ds[r] = p[r] * (ds[r] - d4[e]);
+          }
+        }
+        if (WANT & 1) {
+          const typename F::Rows x(p);
+#pragma unroll
+          for (int j = 0; j < DT; ++j) av[j] = x.template mma<DP>(lg + buf * TILE, 32 * b, j, av[j]);
+        }
+        if (WANT & 2) {
+          const typename F::Rows x(ds);
+#pragma unroll
+          for (int j = 0; j < DT; ++j) ak[j] = x.template mma<DP>(lq + buf * TILE, 32 * b, j, ak[j]);
         }
       }
-      if (WANT & 1) {
-        const typename F::Rows x(p);
-#pragma unroll
-        for (int j = 0; j < DT; ++j) av[j] = x.mma(lg + 32 * b * S, S, 32 * j, av[j]);
-      }
-      if (WANT & 2) {
-        const typename F::Rows x(ds);
-#pragma unroll
-        for (int j = 0; j < DT; ++j) ak[j] = x.mma(lq + 32 * b * S, S, 32 * j, ak[j]);
-      }
     }
+    if (i + SETS < n) store(buf ^ 1);
+    ja_landed();
+  }
+  if constexpr (SETS > 1) {
+    float* sums = reinterpret_cast<float*>(lds);
+    if (WANT & 1) {
+      if (set) ja_give(sums, av);
+      __syncthreads();
+      if (!set) ja_take(sums, av);
+      if (WANT & 2) __syncthreads();
+    }
+    if (WANT & 2) {
+      if (set) ja_give(sums, ak);
+      __syncthreads();
+      if (!set) ja_take(sums, ak);
+    }
+    if (set) return;
   }
   T* krow = dk + (int64_t)(ok ? ki - t.r0 : 0) * a.Hkv * a.d;
   T* vrow = dv + (int64_t)(ok ? ki - t.r0 : 0) * a.Hkv * a.dv;
@@ -203,23 +255,49 @@ __global__ __launch_bounds__(256) void jagged_attn_dkv_kernel(JaggedAttnArgs a) 
   }
 }
 
-template <typename T>
+template <typename T, int DP, int BN, int BQ, bool DMA>
 static void bwd_launch(JaggedAttnArgs a, hipStream_t st) {
+  const dim3 gq((unsigned)(a.slots * a.Hkv * a.group)), gk((unsigned)(a.slots * a.Hkv)), one(256), two(512);
+  // two waves a SIMD leave 256 registers: that does for widths of 128 (query pass, bf16) or 64
+  bool done = false;
+  if constexpr (DP * sizeof(T) <= 256) {
+    if (a.sets == 2) {
+      hipLaunchKernelGGL((jagged_attn_dq_kernel<T, DP, BN, DMA, 2>), gq, two, 0, st, a);
+      done = true;
+    }
+  }
+  if (!done) hipLaunchKernelGGL((jagged_attn_dq_kernel<T, DP, BN, DMA, 1>), gq, one, 0, st, a);
+  a.heads_per_key = a.group;
+  a.group = 1;
+  if constexpr (DP == 64) {
+    if (a.sets_k == 2) {
+      hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, 3, DMA, 2>), gk, two, 0, st, a);
+      return;
+    }
+  }
+  if constexpr (DP <= 128) {
+    hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, 3, DMA, 1>), gk, one, 0, st, a);
+  } else {
+    hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, 1, DMA, 1>), gk, one, 0, st, a);
+    hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, 2, DMA, 1>), gk, one, 0, st, a);
+  }
+}
+template <typename T, bool DMA>
+static void bwd_width(JaggedAttnArgs a, hipStream_t st) {
   const int w = a.d > a.dv ? a.d : a.dv;
   constexpr int BN = sizeof(T) == 2 ? 64 : 32;
   a.slots = jagged_slots(a.rows, a.B, 128);
-  const dim3 gq((unsigned)(a.slots * a.Hkv * a.group)), gk((unsigned)(a.slots * a.Hkv)), block(256);
-  if (w <= 64) {
-    hipLaunchKernelGGL((jagged_attn_dq_kernel<T, 64, BN>), gq, block, 0, st, a);
-    hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, 64, BN, 3>), gk, block, 0, st, a);
-  } else if (w <= 128) {
-    hipLaunchKernelGGL((jagged_attn_dq_kernel<T, 128, 32>), gq, block, 0, st, a);
-    hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, 128, 32, 3>), gk, block, 0, st, a);
-  } else {
-    hipLaunchKernelGGL((jagged_attn_dq_kernel<T, 256, 32>), gq, block, 0, st, a);
-    hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, 256, 32, 1>), gk, block, 0, st, a);
-    hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, 256, 32, 2>), gk, block, 0, st, a);
-  }
+  a.sets_k = (a.rows / 128 + a.B) * a.Hkv <= 2 * device_cus() ? 2 : 1;
+  if (w <= 64)
+    bwd_launch<T, 64, BN, BN, DMA>(a, st);
+  else if (w <= 128)
+    bwd_launch<T, 128, 32, 32, DMA>(a, st);
+  else
+    bwd_launch<T, 256, 32, 32, DMA>(a, st);
+}
+template <typename T>
+static void bwd_any(const JaggedAttnArgs& a, hipStream_t st) {
+  a.dma ? bwd_width<T, true>(a, st) : bwd_width<T, false>(a, st);
 }
 
 }  // namespace gr
@@ -232,7 +310,8 @@ size_t gr_jagged_attn_bwd_workspace_size(int64_t rows, int H) {
 
 int gr_jagged_attn_bwd(const void* q, int64_t ld_q, int64_t hs_q, const void* k, int64_t ld_k, int64_t hs_k,
                        const void* v, int64_t ld_v, int64_t hs_v, const int64_t* offsets, int B, int64_t rows, int H,
-                       int Hkv, int d, int dv, int causal, float scale, int bf16, const void* out, const float* lse,
+                       int Hkv, int d, int dv, int causal, float scale, int bf16, const void* out,
+                       const void* out_low, const float* lse,
                        const void* dout, void* dq, void* dk, void* dvv, void* workspace, size_t ws_bytes, void* stream) {
   gr::JaggedAttnArgs a{};
   a.q = q; a.ld_q = ld_q; a.hs_q = hs_q;
@@ -241,15 +320,14 @@ int gr_jagged_attn_bwd(const void* q, int64_t ld_q, int64_t hs_q, const void* k,
   a.offsets = offsets; a.B = B; a.rows = rows;
   a.Hkv = Hkv; a.d = d; a.dv = dv;
   a.causal = causal; a.scale = scale; a.scale_l2 = scale * 1.44269504f;
-  a.out = const_cast<void*>(out); a.lse = const_cast<float*>(lse);
+  a.out = const_cast<void*>(out); a.out_low = const_cast<void*>(out_low); a.lse = const_cast<float*>(lse);
   a.dout = dout; a.dq = dq; a.dk = dk; a.dvv = dvv; a.delta = (float*)workspace;
-  if (gr::jagged_attn_check("gr_jagged_attn_bwd", a, H)) return 1;
+  if (gr::jagged_attn_check("gr_jagged_attn_bwd", a, H, bf16)) return 1;
   if (rows == 0) return 0;
-  GR_REQUIRE(lse && dout && dq && dk && dvv, "gr_jagged_attn_bwd: null pointer");
+  GR_REQUIRE(lse && dout && (out_low || !bf16) && dq && dk && dvv, "gr_jagged_attn_bwd: null pointer");
   GR_REQUIRE(workspace && ws_bytes >= gr_jagged_attn_bwd_workspace_size(rows, H), "gr_jagged_attn_bwd: workspace too small");
-  a.group = H / Hkv;
   const hipStream_t st = (hipStream_t)stream;
-  GR_TIMED("jagged_attn_bwd", st, bf16 ? gr::bwd_launch<__bf16>(a, st) : gr::bwd_launch<float>(a, st));
+  GR_TIMED("jagged_attn_bwd", st, bf16 ? gr::bwd_any<__bf16>(a, st) : gr::bwd_any<float>(a, st));
   GR_LAUNCH_CHECK("gr_jagged_attn_bwd");
   return 0;
 }

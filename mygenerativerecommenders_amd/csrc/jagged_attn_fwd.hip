@@ -15,127 +15,177 @@
 
 namespace gr {
 
-template <typename T, int DP, int BN>
-__global__ __launch_bounds__(256) void jagged_attn_fwd_kernel(JaggedAttnArgs a) {
+template <typename T, int DP, int BN, bool DMA, int SETS>
+__global__ __launch_bounds__(256 * SETS) void jagged_attn_fwd_kernel(JaggedAttnArgs a) {
   using F = JaFrag<T>;
-  constexpr int BM = 128, NB = BN / 32, DT = DP / 32;
-  constexpr int SK = ja_row_stride<T>(DP), SV = ja_col_stride<T>(DP);
-  __shared__ __attribute__((aligned(16))) T lk[BN * SK];
-  __shared__ __attribute__((aligned(16))) T lv[BN * SV];
-  const int64_t w = blockIdx.x;
-  const int g = (int)(w % a.group);
-  const int64_t ws = w / a.group;
-  const int hk = (int)(ws / a.slots), head = hk * a.group + g;
-  const int H = a.Hkv * a.group;
+  using Tile = JaTile<T, DP>;
+  constexpr int BM = 128, NB = BN / 32, DT = DP / 32, TILE = Tile::size(BN);
+  __shared__ u32x4_t lds[SETS * 4 * TILE];
+  static_assert(SETS == 1 || sizeof(lds) >= (4 * DT * 16 + 8) * 256, "a set's sums fit");
+  const JaggedWork wk = jagged_work(a, blockIdx.x);
+  const int head = wk.hk * a.group + wk.g, H = a.Hkv * a.group;
   // later tiles of a causal sequence have more keys: they go first
-  const JaggedTile t = jagged_tile<BM>(a.offsets, a.B, a.rows, a.slots - 1 - ws % a.slots);
+  const JaggedTile t = jagged_tile<BM>(a.offsets, a.B, a.rows, a.slots - 1 - wk.slot);
   if (t.len == 0) return;
   if (t.tail) {
     ja_zero((T*)a.out + ((t.s0 + t.r0) * H + head) * a.dv, (int64_t)H * a.dv, min(BM, t.len - t.r0), a.dv);
     return;
   }
   const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5;
-  const int q0 = t.r0 + 32 * wave, qi = q0 + (lane & 31);
-  const T* kb = (const T*)a.k + t.s0 * a.ld_k + hk * a.hs_k;
-  const T* vb = (const T*)a.v + t.s0 * a.ld_v + hk * a.hs_v;
+  const int set = SETS > 1 ? wave >> 2 : 0;  // takes tiles set, set + SETS, ..
+  u32x4_t *lk = lds + set * 4 * TILE, *lv = lk + 2 * TILE;
+  const int q0 = t.r0 + 32 * (wave & 3), qi = q0 + (lane & 31);
+  const T* kb = (const T*)a.k + t.s0 * a.ld_k + wk.hk * a.hs_k;
+  const T* vb = (const T*)a.v + t.s0 * a.ld_v + wk.hk * a.hs_v;
   const int keys = a.causal ? min(t.len, t.r0 + BM) : t.len;
-  JaStage<T, DP, BN> sk, sv;
-  sk.load(kb, a.ld_k, 0, t.len, a.d);
-  sv.load(vb, a.ld_v, 0, t.len, a.dv);
+  JaStage<T, DP, BN, DMA> sk, sv;
+  const int first = set * BN, step = SETS * BN;
+  if (first < keys) {
+    sk.load(kb, a.ld_k, first, t.len, a.d, lk);
+    sv.load(vb, a.ld_v, first, t.len, a.dv, lv);
+  }
   JaRows<T, DP, ja_keep<T, DP>> q;
   q.init((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, a.ld_q, q0, t.len, a.d);
+  if (first < keys) {
+    sk.store(lk, first, t.len, a.d);
+    sv.store(lv, first, t.len, a.dv);
+  }
+  ja_landed();
   f32x16 o[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = f16_zero();
   float m = -INFINITY, l = 0.f;
-  for (int k0 = 0; k0 < keys; k0 += BN) {
-    __syncthreads();
-    sk.store(lk, SK, k0, t.len, a.d);
-    sv.store(lv, SV, k0, t.len, a.dv);
-    __syncthreads();
-    if (k0 + BN < keys) {
-      sk.load(kb, a.ld_k, k0 + BN, t.len, a.d);
-      sv.load(vb, a.ld_v, k0 + BN, t.len, a.dv);
+  // every set makes the same number of rounds, the last one perhaps without a tile
+  for (int k0 = first, buf = 0; k0 - first < keys; k0 += step, buf = TILE - buf) {
+    const bool more = k0 + step < keys;
+    if (more) {
+      sk.load(kb, a.ld_k, k0 + step, t.len, a.d, lk + (TILE - buf));
+      sv.load(vb, a.ld_v, k0 + step, t.len, a.dv, lv + (TILE - buf));
     }
     // a wave whose rows are past the end, or before every key of the tile, has nothing here
-    if (q0 >= t.len || (a.causal && k0 > q0 + 31)) continue;
-    f32x16 s[NB];
+    if (q0 < t.len && k0 < keys && !(a.causal && k0 > q0 + 31)) {
+      f32x16 s[NB];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) s[b] = ja_scores(lk + 32 * b * SK, SK, q);
-    if (k0 + BN > t.len || (a.causal && k0 + BN - 1 > q0)) {
-      const int last = a.causal ? min(t.len - 1, qi) : t.len - 1;
+      for (int b = 0; b < NB; ++b) s[b] = ja_scores(lk + buf, 32 * b, q);
+      if (k0 + BN > t.len || (a.causal && k0 + BN - 1 > q0)) {
+        const int last = a.causal ? min(t.len - 1, qi) : t.len - 1;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (k0 + 32 * b + (r & 3) + 8 * (r >> 2) + 4 * half > last) s[b][r] = -INFINITY;
+      }
+      float top = m;
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (k0 + 32 * b + (r & 3) + 8 * (r >> 2) + 4 * half > last) s[b][r] = -INFINITY;
-    }
-    float top = m;
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
-    top = fmaxf(top, swap_half(top));
-    if (__any(top > m)) {  // rescale only where a maximum moved
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+      top = half_max(top);
       const float f = __builtin_amdgcn_exp2f((m - top) * a.scale_l2);
-      l *= f;
+      m = top;
+      const float mc = m * a.scale_l2;
+      float sum = 0.f;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], a.scale_l2, -mc));
+          sum += s[b][r];
+        }
+      l = l * f + sum;
 #pragma unroll
       for (int i = 0; i < DT; ++i) o[i] *= f;
-      m = top;
-    }
-    const float mc = m * a.scale_l2;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+      for (int b = 0; b < NB; ++b) {
+        const typename F::Rows p(s[b]);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], a.scale_l2, -mc));
-        l += s[b][r];
+        for (int i = 0; i < DT; ++i) o[i] = p.template mma<DP>(lv + buf, 32 * b, i, o[i]);
       }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const typename F::Rows p(s[b]);
-#pragma unroll
-      for (int i = 0; i < DT; ++i) o[i] = p.mma(lv + 32 * b * SV, SV, 32 * i, o[i]);
     }
+    if (more) {
+      sk.store(lk + (TILE - buf), k0 + step, t.len, a.d);
+      sv.store(lv + (TILE - buf), k0 + step, t.len, a.dv);
+    }
+    ja_landed();
   }
-  l += swap_half(l);
+  l = half_sum(l);
+  if constexpr (SETS > 1) {
+    float *sums = reinterpret_cast<float*>(lds), *ml = sums + 4 * DT * 16 * 64 + (wave & 3) * 128 + lane;
+    if (set) {
+      ja_give(sums, o);
+      ml[0] = m;
+      ml[64] = l;
+    }
+    __syncthreads();
+    if (set) return;
+    const float top = fmaxf(m, ml[0]), f = __builtin_amdgcn_exp2f((m - top) * a.scale_l2),
+                g = __builtin_amdgcn_exp2f((ml[0] - top) * a.scale_l2);
+    ja_take(sums, o, f, g);
+    l = l * f + ml[64] * g;
+    m = top;
+  }
   const bool ok = qi < t.len;
-  T* out = (T*)a.out + ((t.s0 + (ok ? qi : 0)) * H + head) * a.dv;
+  const int64_t out0 = ((t.s0 + (ok ? qi : 0)) * H + head) * a.dv;
+  T* low = sizeof(T) == 2 && a.out_low ? (T*)a.out_low + out0 : nullptr;
   const float inv = 1.f / l;
 #pragma unroll
-  for (int i = 0; i < DT; ++i) ja_store_t<T>(out, 32 * i, a.dv, o[i], inv, ok);
+  for (int i = 0; i < DT; ++i) ja_store_t<T>((T*)a.out + out0, 32 * i, a.dv, o[i], inv, ok, low);
   if (a.lse && ok && half == 0) a.lse[head * a.rows + t.s0 + qi] = m * a.scale_l2 + __builtin_amdgcn_logf(l);
 }
 
-int jagged_attn_check(const char* what, const JaggedAttnArgs& a, int H) {
-  GR_REQUIRE(a.B >= 0 && a.rows >= 0 && H >= 1 && a.Hkv >= 1 && H % a.Hkv == 0 && a.d >= 1 && a.d <= 256 &&
-                 a.dv >= 1 && a.dv <= 256,
+int jagged_attn_check(const char* what, JaggedAttnArgs& a, int H, int bf16) {
+  const int least = bf16 ? 8 : 4;  // 16 bytes
+  GR_REQUIRE(a.B >= 0 && a.rows >= 0 && H >= 1 && a.Hkv >= 1 && H % a.Hkv == 0 && a.d >= least && a.d <= 256 &&
+                 a.dv >= least && a.dv <= 256,
              "%s: bad sizes", what);
   GR_REQUIRE(a.scale > 0.f && a.scale < INFINITY, "%s: scale must be positive", what);
   GR_REQUIRE(a.rows == 0 || (a.q && a.k && a.v && a.offsets && a.out), "%s: null pointer", what);
   GR_REQUIRE(a.rows < (1ll << 31) && (a.rows / 32 + a.B + 1) * (int64_t)H < (1ll << 31), "%s: too many tiles", what);
+  const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.dout;
+  const int64_t steps = a.ld_q | a.hs_q | a.ld_k | a.hs_k | a.ld_v | a.hs_v | a.d | a.dv;
+  const int64_t far = (int64_t)1 << 22;  // a tile's byte offsets stay below 2^31
+  a.dma = at % 16 == 0 && steps % least == 0 && a.ld_q < far && a.ld_k < far && a.ld_v < far &&
+          a.ld_q >= a.d && a.ld_k >= a.d && a.ld_v >= a.dv;
+  a.group = H / a.Hkv;
+  const int64_t tiles = (a.rows / 128 + a.B) * H;
+  a.sets = tiles <= 2 * device_cus() ? 2 : 1;
   return 0;
 }
 
-template <typename T>
+template <typename T, int DP, int BN, bool DMA>
+static void fwd_sets(const JaggedAttnArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)(a.slots * a.Hkv * a.group));
+  // two waves a SIMD leave 256 registers: widths of 128 (fp32: 64) at most
+  if constexpr (DP * sizeof(T) <= 256) {
+    if (a.sets == 2) {
+      hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, DP, BN, DMA, 2>), grid, dim3(512), 0, st, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, DP, BN, DMA, 1>), grid, dim3(256), 0, st, a);
+}
+template <typename T, int DP, int BN>
 static void fwd_launch(const JaggedAttnArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)(a.slots * a.Hkv * a.group)), block(256);
+  a.dma ? fwd_sets<T, DP, BN, true>(a, st) : fwd_sets<T, DP, BN, false>(a, st);
+}
+template <typename T>
+static void fwd_width(const JaggedAttnArgs& a, hipStream_t st) {
   const int w = a.d > a.dv ? a.d : a.dv;
   constexpr int BN = sizeof(T) == 2 ? 64 : 32;
   if (w <= 64)
-    hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, 64, BN>), grid, block, 0, st, a);
+    fwd_launch<T, 64, BN>(a, st);
   else if (w <= 128)
-    hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, 128, BN>), grid, block, 0, st, a);
+    fwd_launch<T, 128, BN>(a, st);
   else
-    hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, 256, 32>), grid, block, 0, st, a);
+    fwd_launch<T, 256, 32>(a, st);
 }
 
 }  // namespace gr
 
 extern "C" int gr_jagged_attn_fwd(const void* q, int64_t ld_q, int64_t hs_q, const void* k, int64_t ld_k, int64_t hs_k,
                                   const void* v, int64_t ld_v, int64_t hs_v, const int64_t* offsets, int B, int64_t rows,
-                                  int H, int Hkv, int d, int dv, int causal, float scale, int bf16, void* out, float* lse,
-                                  void* stream) {
+                                  int H, int Hkv, int d, int dv, int causal, float scale, int bf16, void* out,
+                                  void* out_low, float* lse, void* stream) {
   gr::JaggedAttnArgs a{};
   a.q = q; a.ld_q = ld_q; a.hs_q = hs_q;
   a.k = k; a.ld_k = ld_k; a.hs_k = hs_k;
@@ -143,13 +193,12 @@ extern "C" int gr_jagged_attn_fwd(const void* q, int64_t ld_q, int64_t hs_q, con
   a.offsets = offsets; a.B = B; a.rows = rows;
   a.Hkv = Hkv; a.d = d; a.dv = dv;
   a.causal = causal; a.scale = scale; a.scale_l2 = scale * 1.44269504f;
-  a.out = out; a.lse = lse;
-  if (gr::jagged_attn_check("gr_jagged_attn_fwd", a, H)) return 1;
+  a.out = out; a.out_low = out_low; a.lse = lse;
+  if (gr::jagged_attn_check("gr_jagged_attn_fwd", a, H, bf16)) return 1;
   if (rows == 0) return 0;
-  a.group = H / Hkv;
   a.slots = gr::jagged_slots(rows, B, 128);
   const hipStream_t st = (hipStream_t)stream;
-  GR_TIMED("jagged_attn_fwd", st, bf16 ? gr::fwd_launch<__bf16>(a, st) : gr::fwd_launch<float>(a, st));
+  GR_TIMED("jagged_attn_fwd", st, bf16 ? gr::fwd_width<__bf16>(a, st) : gr::fwd_width<float>(a, st));
   GR_LAUNCH_CHECK("gr_jagged_attn_fwd");
   return 0;
 }

@@ -206,6 +206,8 @@ def _on(device):
 
 def _rows_of(x, D: int):
     """x as (rows, D) with contiguous columns: a view wherever its strides allow."""
+    if x.dim() == 2 and x.stride(1) == 1:
+        return x
     x2 = x.reshape(-1, D)
     return x2 if D == 1 or x2.stride(1) == 1 else x2.contiguous()
 
@@ -1298,26 +1300,28 @@ class _JaggedAttention(torch.autograd.Function):
         Hkv, dv = k.shape[1], v.shape[2]
         out = torch.empty(rows, H, dv, dtype=q.dtype, device=q.device)
         lse = torch.empty(H, rows, dtype=torch.float32, device=q.device) if grad_on else None
+        low = torch.empty_like(out) if grad_on and q.dtype == torch.bfloat16 else None
         ctx.call = (offsets.numel() - 1, rows, H, Hkv, d, dv, int(causal), scale,
                     int(q.dtype == torch.bfloat16))
         with _on(q.device):
             _lib.call("gr_jagged_attn_fwd", *_strided(q), *_strided(k), *_strided(v),
-                      offsets.data_ptr(), *ctx.call, out.data_ptr(), _lib.ptr(lse), _stream())
+                      offsets.data_ptr(), *ctx.call, out.data_ptr(), _lib.ptr(low),
+                      _lib.ptr(lse), _stream())
         if grad_on:
-            ctx.save_for_backward(q, k, v, offsets, out, lse)
+            ctx.save_for_backward(q, k, v, offsets, out, low, lse)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, offsets, out, lse = ctx.saved_tensors
+        q, k, v, offsets, out, low, lse = ctx.saved_tensors
         dout = dout.contiguous()
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         n = _lib.lib().gr_jagged_attn_bwd_workspace_size(q.shape[0], q.shape[1])
         ws = torch.empty(max(n, 4), dtype=torch.uint8, device=q.device)
         with _on(q.device):
             _lib.call("gr_jagged_attn_bwd", *_strided(q), *_strided(k), *_strided(v),
-                      offsets.data_ptr(), *ctx.call, out.data_ptr(), lse.data_ptr(),
+                      offsets.data_ptr(), *ctx.call, out.data_ptr(), _lib.ptr(low), lse.data_ptr(),
                       dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(),
                       n, _stream())
         return dq, dk, dv, None, None, None, None
@@ -1361,8 +1365,15 @@ def jagged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     scale = d ** -0.5 if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"jagged_attention: scale must be positive and finite (got {scale})")
+    # the kernels read 16 bytes at a time: narrower heads get zero columns
+    least, dv = (8 if q.dtype == torch.bfloat16 else 4), v.shape[2]
+    if d < least:
+        q, k = (torch.nn.functional.pad(t, (0, least - d)) for t in (q, k))
+    if dv < least:
+        v = torch.nn.functional.pad(v, (0, least - dv))
     grad_on = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v))
-    return _JaggedAttention.apply(q, k, v, offsets.to(torch.int64).contiguous(), bool(causal), scale, grad_on)
+    out = _JaggedAttention.apply(q, k, v, offsets.to(torch.int64).contiguous(), bool(causal), scale, grad_on)
+    return out[..., :dv] if dv < least else out
 
 
 # ------------------------------------------------------------------ cached decoding

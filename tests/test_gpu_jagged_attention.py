@@ -252,10 +252,11 @@ def test_captured_and_replayed(dtype):
 
 def test_rows_beyond_32_bits():
     """Rows whose element offsets pass 2^31 in their buffer: 60,000 rows 40,000 apart, cut into
-    short sequences; the last ones give what a small buffer gives."""
+    short sequences; the last ones against the formula.  (Bits are not compared with a small
+    call's: the number of wave sets that share the sums goes by the number of tiles.)"""
     stride, rows = 40000, 60000
     q, k, v, offsets, dout = make([64, 200], 1, 1, 32, 32, torch.bfloat16)
-    want = run(q, k, v, offsets, dout)
+    ref, lim = reference(q, k, v, offsets, True, 32 ** -0.5, dout)
     big = torch.empty(rows * stride, dtype=torch.bfloat16, device="cuda").view(rows, stride)
     views = []
     for i, t in enumerate((q, k, v)):
@@ -268,8 +269,8 @@ def test_rows_beyond_32_bits():
     ends = torch.cat([cut, torch.tensor([rows - 264, rows - 200, rows], device="cuda")])
     g = torch.zeros(rows, 1, 32, dtype=torch.bfloat16, device="cuda")
     g[rows - 264:] = dout
-    for x, y in zip(run(*views, ends, g), want):
-        assert torch.equal(x[rows - 264:], y)
+    for x, y, e in zip(run(*views, ends, g), ref, lim):
+        assert ((x[rows - 264:].double() - y).abs() <= e).all()
 
 
 def test_refusals():

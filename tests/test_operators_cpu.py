@@ -19,28 +19,28 @@ def attn(**kw):
 
 
 @pytest.mark.parametrize("bad", [dict(q=None), dict(k=None), dict(v=None), dict(offsets=None), dict(B=-1), dict(rows=-1),
-                                 dict(H=0), dict(Hkv=0), dict(H=3, Hkv=2), dict(d=0), dict(d=257), dict(dv=0), dict(dv=300),
+                                 dict(H=0), dict(Hkv=0), dict(H=3, Hkv=2), dict(d=3), dict(d=7, bf16=1), dict(d=257), dict(dv=0), dict(dv=300),
                                  dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
                                  dict(rows=1 << 31), dict(rows=1 << 30, H=4096, Hkv=4096)], ids=str)
 def test_attention_refuses(bad):
     with pytest.raises(_lib.GrError, match="gr_jagged_attn_fwd"):
-        _lib.call("gr_jagged_attn_fwd", *attn(**bad), P, None, None)
+        _lib.call("gr_jagged_attn_fwd", *attn(**bad), P, None, None, None)
     with pytest.raises(_lib.GrError, match="gr_jagged_attn_bwd"):
-        _lib.call("gr_jagged_attn_bwd", *attn(**bad), P, P, P, P, P, P, P, 1 << 40, None)
+        _lib.call("gr_jagged_attn_bwd", *attn(**bad), P, P, P, P, P, P, P, P, 1 << 40, None)
 
 
 def test_attention_backward_refuses_missing_buffers():
-    for i in range(7):
-        bufs = [P] * 7
+    for i in range(8):
+        bufs = [P] * 8
         bufs[i] = None
         with pytest.raises(_lib.GrError):
-            _lib.call("gr_jagged_attn_bwd", *attn(), *bufs, 1 << 20, None)
+            _lib.call("gr_jagged_attn_bwd", *attn(bf16=1), *bufs, 1 << 20, None)
     n = _lib.lib().gr_jagged_attn_bwd_workspace_size(4, 2)
     assert n == 32
     with pytest.raises(_lib.GrError, match="workspace"):
-        _lib.call("gr_jagged_attn_bwd", *attn(), *[P] * 7, n - 1, None)
+        _lib.call("gr_jagged_attn_bwd", *attn(), *[P] * 8, n - 1, None)
     with pytest.raises(_lib.GrError):
-        _lib.call("gr_jagged_attn_fwd", *attn(), None, None, None)
+        _lib.call("gr_jagged_attn_fwd", *attn(), None, None, None, None)
 
 
 def test_layer_norm_refuses():
