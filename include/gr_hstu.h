@@ -286,7 +286,8 @@ GR_API int gr_adamw_step(float* const* params, const float* const* grads, const 
  * (offs[i] + element, step), with the probability of its place between its neighbours, and a
  * nonzero exp_avg_sq never becomes zero.  A block that holds an infinity or NaN gets a NaN
  * scale.  Hyper-parameters are rounded once to fp32 (1 - beta, 1 - lr wd from doubles), the
- * bias corrections computed in double.  One launch per 64 tensors; step and done as above. */
+ * bias corrections computed in double.  One launch per 64 tensors; step as above; done: 1,040
+ * uint32 completion counters, zero before the first call (the kernel re-arms them). */
 GR_API int gr_adamw8_step(float* const* params, const float* const* grads, const int64_t* offs,
                           const int64_t* numel, int n_tensors, uint8_t* exp_avg,
                           float* exp_avg_scale, uint8_t* exp_avg_sq, float* exp_avg_sq_scale,

@@ -14,6 +14,8 @@
 // becomes zero (m / eps would follow); below 2^-9 of the scale, 1/229,376 of the block's
 // largest possible v, it is held at that value, which only shortens the steps of such elements.
 // A block that holds an infinity or NaN gets a NaN scale: its moments are lost visibly.
+#include <cmath>
+
 #include "common.h"
 
 #include "../../include/gr_hstu.h"
@@ -38,7 +40,7 @@ struct AdamW8Args {
   float* v_scale;
   float* step;
   uint32_t* done;
-  double lr, beta1, beta2;
+  double lr, log2_b1, log2_b2;  // beta^t = 2^(t log2 beta): half a power's work
   float b1, c1, b2, c2, keep, eps;  // c = 1 - b, keep = 1 - lr wd, each rounded once from doubles
 };
 
@@ -109,30 +111,22 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamW8Args a) {
 #pragma clang fp contract(off)
   __shared__ float sc[3];
   const int w = blockIdx.x;
-  int t = 0;
-  while (t + 1 < a.n_tensors && a.first_chunk[t + 1] <= w) ++t;  // wave-uniform
+  int t = 0;  // the tensor of chunk w: the last whose first chunk is <= w (wave-uniform)
+  for (int half = ADAMW8_MAX / 2; half >= 1; half /= 2)
+    if (t + half < a.n_tensors && a.first_chunk[t + half] <= w) t += half;
   const int64_t n = a.n[t], off = a.off[t];
   const int64_t c0 = (int64_t)(w - a.first_chunk[t]) * a.chunk;
   const int64_t cend = n < c0 + a.chunk ? n : c0 + a.chunk;
   float* param = a.param[t];
   const float* grad = a.grad[t];
   const bool vec = ((reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
-  if (threadIdx.x == 0) {
-    const float ts = a.step[0] + 1.f;
-    sc[0] = ts;
-    sc[1] = (float)(a.lr / (1.0 - pow(a.beta1, (double)ts)));
-    sc[2] = (float)sqrt(1.0 - pow(a.beta2, (double)ts));
-  }
-  __syncthreads();
-  const float ts = sc[0], size = sc[1], root = sc[2];
-  const uint32_t key = (uint32_t)ts * 0xA54FF53Bu;
-  for (int64_t s0 = c0; s0 < cend; s0 += ADAMW8_SUB) {
-    const int64_t i = s0 + 4 * (int64_t)threadIdx.x;
-    // whole 64-element blocks: the lanes of a tensor's last block past its end carry zeros
-    if (i >= (cend + ADAMW8_BLOCK - 1) / ADAMW8_BLOCK * ADAMW8_BLOCK) continue;
-    float p[4], g[4], m[4], v[4];
-    const bool wide = vec && i + 3 < n;
-    if (wide) {
+  // whole 64-element blocks: the lanes of a tensor's last block past its end carry zeros
+  const int64_t end = (cend + ADAMW8_BLOCK - 1) / ADAMW8_BLOCK * ADAMW8_BLOCK;
+  float p[4], g[4], m[4], v[4], ms, vs;
+  uint32_t mc, vc;
+  auto load = [&](int64_t i) {
+    if (i >= end) return;
+    if (vec && i + 3 < n) {
       const float4 pv = *reinterpret_cast<const float4*>(param + i), gv = *reinterpret_cast<const float4*>(grad + i);
       p[0] = pv.x; p[1] = pv.y; p[2] = pv.z; p[3] = pv.w;
       g[0] = gv.x; g[1] = gv.y; g[2] = gv.z; g[3] = gv.w;
@@ -144,42 +138,69 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamW8Args a) {
       }
     }
     const int64_t at = off + i;
-    decode4(*reinterpret_cast<const uint32_t*>(a.m + at), a.m_scale[at / ADAMW8_BLOCK], m);
-    decode4(*reinterpret_cast<const uint32_t*>(a.v + at), a.v_scale[at / ADAMW8_BLOCK], v);
+    mc = *reinterpret_cast<const uint32_t*>(a.m + at);
+    vc = *reinterpret_cast<const uint32_t*>(a.v + at);
+    ms = a.m_scale[at / ADAMW8_BLOCK];
+    vs = a.v_scale[at / ADAMW8_BLOCK];
+  };
+  int64_t i = c0 + 4 * (int64_t)threadIdx.x;
+  load(i);  // on its way while the step is read
+  if (threadIdx.x == 0) {
+    const float ts = a.step[0] + 1.f;
+    sc[0] = ts;
+    sc[1] = (float)(a.lr / (1.0 - exp2((double)ts * a.log2_b1)));
+    sc[2] = (float)(1.0 / sqrt(1.0 - exp2((double)ts * a.log2_b2)));
+  }
+  __syncthreads();
+  const float ts = sc[0], size = sc[1], root = sc[2];
+  const uint32_t key = (uint32_t)ts * 0xA54FF53Bu;
+  for (; i < end; i += ADAMW8_SUB) {
+    decode4(mc, ms, m);
+    decode4(vc, vs, v);
+    const int64_t at = off + i;
     uint32_t rm[4], rv[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       m[e] = m[e] * a.b1 + g[e] * a.c1;
       v[e] = v[e] * a.b2 + g[e] * g[e] * a.c2;
-      p[e] = p[e] * a.keep - size * (m[e] / (sqrtf(v[e]) / root + a.eps));
+      // square root and reciprocal to one step of fp32 each: the update's error stays some
+      // 1e-7 of a step that is itself a small part of the parameter
+      p[e] = p[e] * a.keep - size * (m[e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[e]) * root + a.eps));
       const uint32_t h = place_bits((uint32_t)at + e, key);
       rm[e] = h & 0xFFFFFu;
       rv[e] = h >> 12;
     }
-    if (wide) {
+    if (vec && i + 3 < n) {
       *reinterpret_cast<float4*>(param + i) = float4{p[0], p[1], p[2], p[3]};
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (i + e < n) param[i + e] = p[e];
     }
-    float ms, vs;
-    const uint32_t mc = encode4<false>(m, rm, ms), vc = encode4<true>(v, rv, vs);
-    *reinterpret_cast<uint32_t*>(a.m + at) = mc;
-    *reinterpret_cast<uint32_t*>(a.v + at) = vc;
+    const uint32_t mn = encode4<false>(m, rm, ms), vn = encode4<true>(v, rv, vs);
+    *reinterpret_cast<uint32_t*>(a.m + at) = mn;
+    *reinterpret_cast<uint32_t*>(a.v + at) = vn;
     if ((threadIdx.x & 15) == 0) {
       a.m_scale[at / ADAMW8_BLOCK] = ms;
       a.v_scale[at / ADAMW8_BLOCK] = vs;
     }
+    load(i + ADAMW8_SUB);
   }
   if (!a.advance) return;
-  // the last workgroup to finish writes the step and re-arms the counter; relaxed, as the
-  // increment only has to follow this workgroup's read of the step (consumed before the
-  // barrier above)
-  if (threadIdx.x == 0 &&
-      __hip_atomic_fetch_add(a.done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1) {
-    a.step[0] = ts;
-    __hip_atomic_store(a.done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  // The last workgroup to finish writes the step and re-arms the counters.  Workgroups count
+  // in 64 groups and the last of each group once more: one counter for all is a queue of
+  // some 10 ns a workgroup (2,660 of them: 36 us against 13).  Relaxed: an increment only
+  // has to follow its workgroup's read of the step (consumed before the barrier above).
+  if (threadIdx.x == 0) {
+    const uint32_t n = gridDim.x, k = blockIdx.x % 64, mine = n / 64 + (k < n % 64), groups = n < 64 ? n : 64;
+    uint32_t* sub = a.done + 16 * (1 + k);
+    if (__hip_atomic_fetch_add(sub, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == mine - 1) {
+      __hip_atomic_store(sub, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (__hip_atomic_fetch_add(a.done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == groups - 1) {
+        a.step[0] = ts;
+        __hip_atomic_store(a.done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    }
   }
 }
 }  // namespace gr
@@ -218,8 +239,8 @@ extern "C" int gr_adamw8_step(float* const* params, const float* const* grads, c
   a.step = step;
   a.done = done;
   a.lr = lr;
-  a.beta1 = beta1;
-  a.beta2 = beta2;
+  a.log2_b1 = std::log2(beta1);  // beta = 0: -inf, and 2^(t log2 beta) = 0
+  a.log2_b2 = std::log2(beta2);
   a.b1 = (float)beta1;
   a.c1 = (float)(1.0 - beta1);
   a.b2 = (float)beta2;

@@ -90,7 +90,7 @@ class FlatAdamW(torch.optim.Optimizer):
                              "exp_avg_scale": fs["exp_avg_scale"][blocks],
                              "exp_avg_sq": fs["exp_avg_sq"][off:off + n].view_as(p),
                              "exp_avg_sq_scale": fs["exp_avg_sq_scale"][blocks]}
-        fs["done"] = torch.zeros(1, dtype=torch.int32, device=dev)
+        fs["done"] = torch.zeros(1040, dtype=torch.int32, device=dev)  # 65 counters, 64 bytes apart
         fs["offs"] = offs
         self._flat[gi] = fs
         return fs
