@@ -318,8 +318,9 @@ GR_API int gr_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64
  * offsets[b + 1]), keys j <= i only where causal:
  *   out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h']) v[j, h'],  h' = h / (H / Hkv)
  * q (rows, H, d), k (rows, Hkv, d), v (rows, Hkv, dv): bf16 (bf16 != 0) or fp32, element
- * strides ld_* of a row and hs_* of a head, columns contiguous, no alignment beyond the
- * element's; 16 bytes <= d, dv <= 256 elements, H a multiple of Hkv, scale > 0.  out, dout (rows, H, dv), dq
+ * strides ld_* of a row (in [0, 2^22)) and hs_* of a head, columns contiguous, no alignment
+ * beyond the element's for fp32, even strides and widths from 4-byte boundaries on for bf16;
+ * 16 bytes <= d, dv <= 256 elements, H a multiple of Hkv, scale > 0.  out, dout (rows, H, dv), dq
  * (rows, H, d), dk (rows, Hkv, d), dvv (rows, Hkv, dv) are contiguous.  Rows past
  * offsets[B] get zeros; offsets are clamped to [0, rows].  lse (H, rows): log2 of each row's
  * sum of exp(scaled scores); out_low (bf16 only, as out): what rounding left off out, so that

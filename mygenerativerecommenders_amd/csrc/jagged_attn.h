@@ -37,7 +37,7 @@ struct JaggedAttnArgs {
   void* dvv;         // (rows, Hkv, dv)
   float* delta;      // (H, rows): sum(dout * out)
   int64_t slots;     // tiles of the rows per head, see jagged_tile
-  int dma;           // rows can go straight to LDS
+  int wide;          // rows and their starts are multiples of 16 bytes
   int heads_per_key; // the backward's key pass: `group`, where that is 1 for its grid
   int sets, sets_k;  // sets of four waves that share a workgroup's tiles (1 or 2), query and key pass
 };
@@ -146,62 +146,44 @@ struct JaTile {
            (c0 & ~BITS) + size(r0);
   }
 };
-// Brings R rows of a jagged operand into an LDS tile, with a set of four waves.  DMA: straight from
-// memory (buffer_load_dwordx4 to LDS; rows of a multiple of 16 bytes, 16-byte aligned), issued
-// where the compiler does not see it, so that it does not wait for it at the next LDS read:
-// ja_landed() waits and meets the other waves.  The descriptor ends with the sequence's last
-// row, so rows past it come as zeros.  Otherwise through registers.
-template <typename T, int DP, int R, bool DMA>
-struct JaStage;
-template <typename T, int DP, int R>
-struct JaStage<T, DP, R, true> {
+// Brings R rows of a jagged operand into an LDS tile, with a set of four waves, straight from
+// memory (buffer loads to LDS of BYTES a lane: 16 where rows and their starts are multiples of
+// that, else 4).  They are issued where the compiler does not see them, so that it does not
+// wait for them at the next LDS read: ja_landed() waits and meets the other waves.  The
+// descriptor ends with the sequence's last row, so rows past it come as zeros, and lanes past
+// column d ask for what is out of its range.
+template <typename T, int DP, int R, int BYTES>
+__device__ __forceinline__ void ja_stage(const T* base, int64_t ld, int r0, int len, int d, u32x4_t* tile) {
   using Tile = JaTile<T, DP>;
-  static constexpr int N = R * Tile::UNITS / 256;  // instructions of a wave
+  constexpr int SZ = sizeof(T), PER = 16 / BYTES;             // lanes that share a unit
+  constexpr int N = R * Tile::UNITS * PER / 256;              // instructions of a wave
+  constexpr int STEP = BYTES == 16 ? 4 * Tile::RPI : Tile::RPI;  // rows from one to its next
   static_assert(R * Tile::UNITS % 256 == 0 && Tile::UNITS <= 64, "whole instructions");
-  __device__ __forceinline__ void load(const T* base, int64_t ld, int r0, int len, int d, u32x4_t* tile) {
-    constexpr int SZ = sizeof(T);
-    const int lane = threadIdx.x & 63, r = (wave_id() & 3) * Tile::RPI + lane / Tile::UNITS;
-    const int c = (lane % Tile::UNITS ^ Tile::swizzle(r)) * Tile::V;
-    const uint32_t at = __builtin_amdgcn_readfirstlane(
-        (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u32x4_t*)tile + 1040u * (wave_id() & 3));
-    const uint64_t p = (uint64_t)(base + (int64_t)r0 * ld);
-    const int64_t bytes = ((int64_t)(len - r0 - 1) * ld + d) * SZ;
-    const u32x4_t desc = {(uint32_t)p, (uint32_t)(p >> 32) & 0xFFFFu, (uint32_t)(bytes < 0x7FFFFFFF ? bytes : 0x7FFFFFFF),
-                          0x00020000u};
-    const uint32_t off = c < d ? (uint32_t)(r * (int)ld + c) * SZ : (uint32_t)OOB_OFF;  // ld < 2^22
+  const int lane = threadIdx.x & 63, w = wave_id() & 3;
+  const int u = w * 64 / PER + lane / PER, r = u / Tile::UNITS;  // unit of the set's first 4 instructions
+  const int c = (u % Tile::UNITS ^ Tile::swizzle(r)) * Tile::V + lane % PER * (BYTES / SZ);
+  const uint32_t at = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u32x4_t*)tile + (BYTES == 16 ? 1040u : 256u) * w);
+  const uint64_t p = (uint64_t)(base + (int64_t)r0 * ld);
+  const int64_t bytes = ((int64_t)(len - r0 - 1) * ld + d) * SZ;
+  const u32x4_t desc = {(uint32_t)p, (uint32_t)(p >> 32) & 0xFFFFu, (uint32_t)(bytes < 0x7FFFFFFF ? bytes : 0x7FFFFFFF),
+                        0x00020000u};
+  const uint32_t off = c < d ? (uint32_t)(r * (int)ld + c) * SZ : (uint32_t)OOB_OFF;  // ld < 2^22
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      uint32_t keep;
+  for (int i = 0; i < N; ++i) {
+    uint32_t keep;
+    const uint32_t to = at + (BYTES == 16 ? 4160u : 1040u) * i;
+    const int from = STEP * SZ * i * (int)ld;
+    if constexpr (BYTES == 16)
       asm volatile(
           "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
-          : "=&s"(keep)
-          : "s"(at + 4160u * i), "v"(off), "s"(desc), "s"(4 * Tile::RPI * SZ * i * (int)ld)
-          : "memory");
-    }
+          : "=&s"(keep) : "s"(to), "v"(off), "s"(desc), "s"(from) : "memory");
+    else
+      asm volatile(
+          "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
+          : "=&s"(keep) : "s"(to), "v"(off), "s"(desc), "s"(from) : "memory");
   }
-  __device__ __forceinline__ void store(u32x4_t*, int, int, int) {}
-};
-template <typename T, int DP, int R>
-struct JaStage<T, DP, R, false> {
-  using Tile = JaTile<T, DP>;
-  static constexpr int N = R * Tile::UNITS / 256;
-  static_assert(R * Tile::UNITS % 256 == 0, "whole passes");
-  u32x4_t x[N];
-  __device__ __forceinline__ void load(const T* base, int64_t ld, int r0, int len, int d, u32x4_t*) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = (threadIdx.x & 255) + 256 * i;
-      x[i] = ja_load16<T>(base + (int64_t)min(r0 + at / Tile::UNITS, len - 1) * ld, at % Tile::UNITS * Tile::V, d);
-    }
-  }
-  __device__ __forceinline__ void store(u32x4_t* tile, int r0, int len, int d) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = (threadIdx.x & 255) + 256 * i, r = at / Tile::UNITS, c = at % Tile::UNITS;
-      tile[r / Tile::RPI * 65 + r % Tile::RPI * Tile::UNITS + (c ^ Tile::swizzle(r))] = ja_fix16<T>(x[i], c * Tile::V, d, r0 + r < len);
-    }
-  }
-};
+}
 __device__ __forceinline__ void ja_landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Operand fragments.  `K` contraction steps of a fragment: 16 (bf16) or 8 (fp32); lane half

@@ -16,7 +16,7 @@
 namespace gr {
 
 // dQ: one workgroup per 128 query rows and head, a wave per 32 rows, tiles of BN keys.
-template <typename T, int DP, int BN, bool DMA, int SETS>
+template <typename T, int DP, int BN, int BYTES, int SETS>
 __global__ __launch_bounds__(256 * SETS) void jagged_attn_dq_kernel(JaggedAttnArgs a) {
   using F = JaFrag<T>;
   using Tile = JaTile<T, DP>;
@@ -40,12 +40,12 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_dq_kernel(JaggedAttnAr
   const T* kb = (const T*)a.k + t.s0 * a.ld_k + wk.hk * a.hs_k;
   const T* vb = (const T*)a.v + t.s0 * a.ld_v + wk.hk * a.hs_v;
   const int keys = a.causal ? min(t.len, t.r0 + BM) : t.len;
-  JaStage<T, DP, BN, DMA> sk, sv;
   const int first = set * BN, step = SETS * BN;
-  if (first < keys) {
-    sk.load(kb, a.ld_k, first, t.len, a.d, lk);
-    sv.load(vb, a.ld_v, first, t.len, a.dv, lv);
-  }
+  auto load = [&](int k0, int buf) {
+    ja_stage<T, DP, BN, BYTES>(kb, a.ld_k, k0, t.len, a.d, lk + buf);
+    ja_stage<T, DP, BN, BYTES>(vb, a.ld_v, k0, t.len, a.dv, lv + buf);
+  };
+  if (first < keys) load(first, 0);
   JaRows<T, DP, ja_keep<T, DP>> q, go;
   q.init((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, a.ld_q, q0, t.len, a.d);
   const int64_t out0 = (t.s0 * H + head) * a.dv;
@@ -72,17 +72,9 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_dq_kernel(JaggedAttnAr
   f32x16 acc[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) acc[i] = f16_zero();
-  if (first < keys) {
-    sk.store(lk, first, t.len, a.d);
-    sv.store(lv, first, t.len, a.dv);
-  }
   ja_landed();
   for (int k0 = first, buf = 0; k0 - first < keys; k0 += step, buf = TILE - buf) {
-    const bool more = k0 + step < keys;
-    if (more) {
-      sk.load(kb, a.ld_k, k0 + step, t.len, a.d, lk + (TILE - buf));
-      sv.load(vb, a.ld_v, k0 + step, t.len, a.dv, lv + (TILE - buf));
-    }
+    if (k0 + step < keys) load(k0 + step, TILE - buf);
     if (q0 < t.len && k0 < keys && !(a.causal && k0 > q0 + 31)) {
       const bool edge = k0 + BN > t.len || (a.causal && k0 + BN - 1 > q0);
       const int last = a.causal ? min(t.len - 1, qi) : t.len - 1;
@@ -100,10 +92,6 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_dq_kernel(JaggedAttnAr
 #pragma unroll
         for (int i = 0; i < DT; ++i) acc[i] = ds.template mma<DP>(lk + buf, 32 * b, i, acc[i]);
       }
-    }
-    if (more) {
-      sk.store(lk + (TILE - buf), k0 + step, t.len, a.d);
-      sv.store(lv + (TILE - buf), k0 + step, t.len, a.dv);
     }
     ja_landed();
   }
@@ -123,7 +111,7 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_dq_kernel(JaggedAttnAr
 // rows of each query head of the group in turn.  WANT: 1 = dV, 2 = dK, 3 = both in one launch;
 // heads wider than 128 take a launch for each, as both results' accumulators and the
 // keys' fragments do not fit the registers together.
-template <typename T, int DP, int BQ, int WANT, bool DMA, int SETS>
+template <typename T, int DP, int BQ, int WANT, int BYTES, int SETS>
 __global__ __launch_bounds__(256 * SETS) void jagged_attn_dkv_kernel(JaggedAttnArgs a) {
   using F = JaFrag<T>;
   using Tile = JaTile<T, DP>;
@@ -149,7 +137,6 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_dkv_kernel(JaggedAttnA
   const int k0 = t.r0 + 32 * (wave & 3), ki = k0 + (lane & 31);
   const bool ok = ki < t.len;
   const int first = a.causal ? t.r0 : 0, per = (t.len - first + BQ - 1) / BQ, n = per * group;
-  JaStage<T, DP, BQ, DMA> sq, sg;
   float rl = 0.f, rd = 0.f;
   int r0 = first, head = hk * group;  // the tile last loaded: query rows r0 on of a head
   auto next = [&]() {
@@ -161,8 +148,9 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_dkv_kernel(JaggedAttnA
   };
   if (set) next();  // a set takes every other tile
   auto load = [&](int buf) {
-    sq.load((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, a.ld_q, r0, t.len, a.d, lq + buf * TILE);
-    sg.load((const T*)a.dout + (t.s0 * H + head) * a.dv, (int64_t)H * a.dv, r0, t.len, a.dv, lg + buf * TILE);
+    ja_stage<T, DP, BQ, BYTES>((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, a.ld_q, r0, t.len, a.d, lq + buf * TILE);
+    ja_stage<T, DP, BQ, BYTES>((const T*)a.dout + (t.s0 * H + head) * a.dv, (int64_t)H * a.dv, r0, t.len, a.dv,
+                               lg + buf * TILE);
     if (tid < BQ) {
       const int r = r0 + tid;
       rl = r < t.len ? a.lse[head * a.rows + t.s0 + r] : INFINITY;  // no probability
@@ -170,8 +158,6 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_dkv_kernel(JaggedAttnA
     }
   };
   auto store = [&](int buf) {
-    sq.store(lq + buf * TILE, r0, t.len, a.d);
-    sg.store(lg + buf * TILE, r0, t.len, a.dv);
     if (tid < BQ) {
       ll[buf * BQ + tid] = rl;
       ld[buf * BQ + tid] = rd;
@@ -255,49 +241,49 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_dkv_kernel(JaggedAttnA
   }
 }
 
-template <typename T, int DP, int BN, int BQ, bool DMA>
+template <typename T, int DP, int BN, int BQ, int BYTES>
 static void bwd_launch(JaggedAttnArgs a, hipStream_t st) {
   const dim3 gq((unsigned)(a.slots * a.Hkv * a.group)), gk((unsigned)(a.slots * a.Hkv)), one(256), two(512);
   // two waves a SIMD leave 256 registers: that does for widths of 128 (query pass, bf16) or 64
   bool done = false;
   if constexpr (DP * sizeof(T) <= 256) {
     if (a.sets == 2) {
-      hipLaunchKernelGGL((jagged_attn_dq_kernel<T, DP, BN, DMA, 2>), gq, two, 0, st, a);
+      hipLaunchKernelGGL((jagged_attn_dq_kernel<T, DP, BN, BYTES, 2>), gq, two, 0, st, a);
       done = true;
     }
   }
-  if (!done) hipLaunchKernelGGL((jagged_attn_dq_kernel<T, DP, BN, DMA, 1>), gq, one, 0, st, a);
+  if (!done) hipLaunchKernelGGL((jagged_attn_dq_kernel<T, DP, BN, BYTES, 1>), gq, one, 0, st, a);
   a.heads_per_key = a.group;
   a.group = 1;
   if constexpr (DP == 64) {
     if (a.sets_k == 2) {
-      hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, 3, DMA, 2>), gk, two, 0, st, a);
+      hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, 3, BYTES, 2>), gk, two, 0, st, a);
       return;
     }
   }
   if constexpr (DP <= 128) {
-    hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, 3, DMA, 1>), gk, one, 0, st, a);
+    hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, 3, BYTES, 1>), gk, one, 0, st, a);
   } else {
-    hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, 1, DMA, 1>), gk, one, 0, st, a);
-    hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, 2, DMA, 1>), gk, one, 0, st, a);
+    hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, 1, BYTES, 1>), gk, one, 0, st, a);
+    hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, 2, BYTES, 1>), gk, one, 0, st, a);
   }
 }
-template <typename T, bool DMA>
+template <typename T, int BYTES>
 static void bwd_width(JaggedAttnArgs a, hipStream_t st) {
   const int w = a.d > a.dv ? a.d : a.dv;
   constexpr int BN = sizeof(T) == 2 ? 64 : 32;
   a.slots = jagged_slots(a.rows, a.B, 128);
   a.sets_k = (a.rows / 128 + a.B) * a.Hkv <= 2 * device_cus() ? 2 : 1;
   if (w <= 64)
-    bwd_launch<T, 64, BN, BN, DMA>(a, st);
+    bwd_launch<T, 64, BN, BN, BYTES>(a, st);
   else if (w <= 128)
-    bwd_launch<T, 128, 32, 32, DMA>(a, st);
+    bwd_launch<T, 128, 32, 32, BYTES>(a, st);
   else
-    bwd_launch<T, 256, 32, 32, DMA>(a, st);
+    bwd_launch<T, 256, 32, 32, BYTES>(a, st);
 }
 template <typename T>
 static void bwd_any(const JaggedAttnArgs& a, hipStream_t st) {
-  a.dma ? bwd_width<T, true>(a, st) : bwd_width<T, false>(a, st);
+  a.wide ? bwd_width<T, 16>(a, st) : bwd_width<T, 4>(a, st);
 }
 
 }  // namespace gr

@@ -15,7 +15,7 @@
 
 namespace gr {
 
-template <typename T, int DP, int BN, bool DMA, int SETS>
+template <typename T, int DP, int BN, int BYTES, int SETS>
 __global__ __launch_bounds__(256 * SETS) void jagged_attn_fwd_kernel(JaggedAttnArgs a) {
   using F = JaFrag<T>;
   using Tile = JaTile<T, DP>;
@@ -38,18 +38,14 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_fwd_kernel(JaggedAttnA
   const T* kb = (const T*)a.k + t.s0 * a.ld_k + wk.hk * a.hs_k;
   const T* vb = (const T*)a.v + t.s0 * a.ld_v + wk.hk * a.hs_v;
   const int keys = a.causal ? min(t.len, t.r0 + BM) : t.len;
-  JaStage<T, DP, BN, DMA> sk, sv;
   const int first = set * BN, step = SETS * BN;
-  if (first < keys) {
-    sk.load(kb, a.ld_k, first, t.len, a.d, lk);
-    sv.load(vb, a.ld_v, first, t.len, a.dv, lv);
-  }
+  auto load = [&](int k0, int buf) {
+    ja_stage<T, DP, BN, BYTES>(kb, a.ld_k, k0, t.len, a.d, lk + buf);
+    ja_stage<T, DP, BN, BYTES>(vb, a.ld_v, k0, t.len, a.dv, lv + buf);
+  };
+  if (first < keys) load(first, 0);
   JaRows<T, DP, ja_keep<T, DP>> q;
   q.init((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, a.ld_q, q0, t.len, a.d);
-  if (first < keys) {
-    sk.store(lk, first, t.len, a.d);
-    sv.store(lv, first, t.len, a.dv);
-  }
   ja_landed();
   f32x16 o[DT];
 #pragma unroll
@@ -57,11 +53,7 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_fwd_kernel(JaggedAttnA
   float m = -INFINITY, l = 0.f;
   // every set makes the same number of rounds, the last one perhaps without a tile
   for (int k0 = first, buf = 0; k0 - first < keys; k0 += step, buf = TILE - buf) {
-    const bool more = k0 + step < keys;
-    if (more) {
-      sk.load(kb, a.ld_k, k0 + step, t.len, a.d, lk + (TILE - buf));
-      sv.load(vb, a.ld_v, k0 + step, t.len, a.dv, lv + (TILE - buf));
-    }
+    if (k0 + step < keys) load(k0 + step, TILE - buf);
     // a wave whose rows are past the end, or before every key of the tile, has nothing here
     if (q0 < t.len && k0 < keys && !(a.causal && k0 > q0 + 31)) {
       f32x16 s[NB];
@@ -102,10 +94,6 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_fwd_kernel(JaggedAttnA
         for (int i = 0; i < DT; ++i) o[i] = p.template mma<DP>(lv + buf, 32 * b, i, o[i]);
       }
     }
-    if (more) {
-      sk.store(lk + (TILE - buf), k0 + step, t.len, a.d);
-      sv.store(lv + (TILE - buf), k0 + step, t.len, a.dv);
-    }
     ja_landed();
   }
   l = half_sum(l);
@@ -143,30 +131,33 @@ int jagged_attn_check(const char* what, JaggedAttnArgs& a, int H, int bf16) {
   GR_REQUIRE(a.rows < (1ll << 31) && (a.rows / 32 + a.B + 1) * (int64_t)H < (1ll << 31), "%s: too many tiles", what);
   const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.dout;
   const int64_t steps = a.ld_q | a.hs_q | a.ld_k | a.hs_k | a.ld_v | a.hs_v | a.d | a.dv;
+  // LDS loads of 4 or 16 bytes: bf16 rows of even widths and strides on 4-byte boundaries
   const int64_t far = (int64_t)1 << 22;  // a tile's byte offsets stay below 2^31
-  a.dma = at % 16 == 0 && steps % least == 0 && a.ld_q < far && a.ld_k < far && a.ld_v < far &&
-          a.ld_q >= a.d && a.ld_k >= a.d && a.ld_v >= a.dv;
+  GR_REQUIRE(at % 4 == 0 && (!bf16 || steps % 2 == 0), "%s: bf16 rows must be pairs on 4-byte boundaries", what);
+  GR_REQUIRE(a.rows == 0 || (a.ld_q >= 0 && a.ld_q < far && a.ld_k >= 0 && a.ld_k < far && a.ld_v >= 0 && a.ld_v < far),
+             "%s: row strides outside [0, 2^22)", what);
+  a.wide = at % 16 == 0 && steps % least == 0;
   a.group = H / a.Hkv;
   const int64_t tiles = (a.rows / 128 + a.B) * H;
   a.sets = tiles <= 2 * device_cus() ? 2 : 1;
   return 0;
 }
 
-template <typename T, int DP, int BN, bool DMA>
+template <typename T, int DP, int BN, int BYTES>
 static void fwd_sets(const JaggedAttnArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)(a.slots * a.Hkv * a.group));
   // two waves a SIMD leave 256 registers: widths of 128 (fp32: 64) at most
   if constexpr (DP * sizeof(T) <= 256) {
     if (a.sets == 2) {
-      hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, DP, BN, DMA, 2>), grid, dim3(512), 0, st, a);
+      hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, DP, BN, BYTES, 2>), grid, dim3(512), 0, st, a);
       return;
     }
   }
-  hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, DP, BN, DMA, 1>), grid, dim3(256), 0, st, a);
+  hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, DP, BN, BYTES, 1>), grid, dim3(256), 0, st, a);
 }
 template <typename T, int DP, int BN>
 static void fwd_launch(const JaggedAttnArgs& a, hipStream_t st) {
-  a.dma ? fwd_sets<T, DP, BN, true>(a, st) : fwd_sets<T, DP, BN, false>(a, st);
+  a.wide ? fwd_sets<T, DP, BN, 16>(a, st) : fwd_sets<T, DP, BN, 4>(a, st);
 }
 template <typename T>
 static void fwd_width(const JaggedAttnArgs& a, hipStream_t st) {

@@ -1289,7 +1289,13 @@ def stu_softmax_layer(x, offsets, bias, w_uvqk, w_o, b_o, geo: STUGeometry, seed
 # ------------------------------------------------------------------ per-head softmax attention
 
 def _columns(x):
-    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+    """x itself where the kernels read it in place: contiguous columns, row strides below 2^22,
+    for bfloat16 even strides and a start on a 4-byte boundary; else a contiguous copy."""
+    s = x.stride()
+    ok = s[2] == 1 and 0 <= s[0] < 1 << 22
+    if x.dtype == torch.bfloat16:
+        ok = ok and s[0] % 2 == 0 and s[1] % 2 == 0 and x.data_ptr() % 4 == 0
+    return x if ok else x.contiguous()
 
 
 class _JaggedAttention(torch.autograd.Function):
@@ -1365,15 +1371,18 @@ def jagged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     scale = d ** -0.5 if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"jagged_attention: scale must be positive and finite (got {scale})")
-    # the kernels read 16 bytes at a time: narrower heads get zero columns
-    least, dv = (8 if q.dtype == torch.bfloat16 else 4), v.shape[2]
-    if d < least:
-        q, k = (torch.nn.functional.pad(t, (0, least - d)) for t in (q, k))
-    if dv < least:
-        v = torch.nn.functional.pad(v, (0, least - dv))
+    # heads narrower than 16 bytes, and bf16 heads of odd widths, get zero columns
+    dv = v.shape[2]
+    q, k, v = _even(q, d), _even(k, d), _even(v, dv)
     grad_on = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v))
     out = _JaggedAttention.apply(q, k, v, offsets.to(torch.int64).contiguous(), bool(causal), scale, grad_on)
-    return out[..., :dv] if dv < least else out
+    return out if out.shape[2] == dv else out[..., :dv]
+
+
+def _even(x, d: int):
+    least, even = (8, 2) if x.dtype == torch.bfloat16 else (4, 1)
+    want = max(least, -(-d // even) * even)
+    return x if want == d else torch.nn.functional.pad(x, (0, want - d))
 
 
 # ------------------------------------------------------------------ cached decoding
