@@ -39,7 +39,6 @@ struct JaggedAttnArgs {
   int64_t slots;     // tiles of the rows per head, see jagged_tile
   int wide;          // rows and their starts are multiples of 16 bytes
   int heads_per_key; // the backward's key pass: `group`, where that is 1 for its grid
-  int sets, sets_k;  // sets of four waves that share a workgroup's tiles (1 or 2), query and key pass
 };
 
 // Work item of a workgroup.  Workgroups i, i + 8, .. land on one XCD: each XCD takes a
@@ -146,42 +145,49 @@ struct JaTile {
            (c0 & ~BITS) + size(r0);
   }
 };
-// Brings R rows of a jagged operand into an LDS tile, with a set of four waves, straight from
+// Brings R rows of a jagged operand into an LDS tile, with a set of QW waves, straight from
 // memory (buffer loads to LDS of BYTES a lane: 16 where rows and their starts are multiples of
 // that, else 4).  They are issued where the compiler does not see them, so that it does not
 // wait for them at the next LDS read: ja_landed() waits and meets the other waves.  The
 // descriptor ends with the sequence's last row, so rows past it come as zeros, and lanes past
 // column d ask for what is out of its range.
-template <typename T, int DP, int R, int BYTES>
+template <typename T, int DP, int R, int BYTES, int QW>
 __device__ __forceinline__ void ja_stage(const T* base, int64_t ld, int r0, int len, int d, u32x4_t* tile) {
   using Tile = JaTile<T, DP>;
   constexpr int SZ = sizeof(T), PER = 16 / BYTES;             // lanes that share a unit
-  constexpr int N = R * Tile::UNITS * PER / 256;              // instructions of a wave
-  constexpr int STEP = BYTES == 16 ? 4 * Tile::RPI : Tile::RPI;  // rows from one to its next
-  static_assert(R * Tile::UNITS % 256 == 0 && Tile::UNITS <= 64, "whole instructions");
-  const int lane = threadIdx.x & 63, w = wave_id() & 3;
-  const int u = w * 64 / PER + lane / PER, r = u / Tile::UNITS;  // unit of the set's first 4 instructions
-  const int c = (u % Tile::UNITS ^ Tile::swizzle(r)) * Tile::V + lane % PER * (BYTES / SZ);
+  constexpr int N = R * Tile::UNITS * PER / (64 * QW);        // instructions of a wave
+  // an instruction writes 1 / PER of a kilobyte of the tile; the waves take them in turn, so a
+  // wave meets PH different parts of a kilobyte, each with its own columns
+  constexpr int PH = PER > QW ? PER / QW : 1, BLOCKS = QW > PER ? QW / PER : 1;  // kilobytes a turn
+  static_assert(R * Tile::UNITS * PER % (64 * QW) == 0 && Tile::UNITS <= 64, "whole instructions");
+  const int lane = threadIdx.x & 63, w = wave_id() % QW;
+  uint32_t off[PH];
+#pragma unroll
+  for (int i = 0; i < PH; ++i) {
+    const int u = (i * QW + w) * 64 / PER + lane / PER, r = u / Tile::UNITS;
+    const int c = (u % Tile::UNITS ^ Tile::swizzle(r)) * Tile::V + lane % PER * (BYTES / SZ);
+    off[i] = c < d ? (uint32_t)(r * (int)ld + c) * SZ : (uint32_t)OOB_OFF;  // ld < 2^22
+  }
   const uint32_t at = __builtin_amdgcn_readfirstlane(
-      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u32x4_t*)tile + (BYTES == 16 ? 1040u : 256u) * w);
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u32x4_t*)tile + 1040u * (w / PER) + 1024u / PER * (w % PER));
   const uint64_t p = (uint64_t)(base + (int64_t)r0 * ld);
   const int64_t bytes = ((int64_t)(len - r0 - 1) * ld + d) * SZ;
   const u32x4_t desc = {(uint32_t)p, (uint32_t)(p >> 32) & 0xFFFFu, (uint32_t)(bytes < 0x7FFFFFFF ? bytes : 0x7FFFFFFF),
                         0x00020000u};
-  const uint32_t off = c < d ? (uint32_t)(r * (int)ld + c) * SZ : (uint32_t)OOB_OFF;  // ld < 2^22
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     uint32_t keep;
-    const uint32_t to = at + (BYTES == 16 ? 4160u : 1040u) * i;
-    const int from = STEP * SZ * i * (int)ld;
+    const int turn = i / PH;
+    const uint32_t to = at + 1040u * BLOCKS * turn + (i % PH) * (1024u / PER * QW);
+    const int from = BLOCKS * Tile::RPI * SZ * turn * (int)ld;
     if constexpr (BYTES == 16)
       asm volatile(
           "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
-          : "=&s"(keep) : "s"(to), "v"(off), "s"(desc), "s"(from) : "memory");
+          : "=&s"(keep) : "s"(to), "v"(off[i % PH]), "s"(desc), "s"(from) : "memory");
     else
       asm volatile(
           "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
-          : "=&s"(keep) : "s"(to), "v"(off), "s"(desc), "s"(from) : "memory");
+          : "=&s"(keep) : "s"(to), "v"(off[i % PH]), "s"(desc), "s"(from) : "memory");
   }
 }
 __device__ __forceinline__ void ja_landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -349,17 +355,17 @@ __device__ __forceinline__ void ja_zero(T* base, int64_t ld, int n, int width) {
 
 // Two sets of waves that each took every other tile join their sums: the second set's
 // accumulators pass through LDS (4 KB a tile and wave; the tiles' own space).
-template <int DT>
+template <int QW, int DT>
 __device__ __forceinline__ void ja_give(float* lds, const f32x16 (&v)[DT]) {
-  float* at = lds + ((wave_id() & 3) * DT * 16) * 64 + (threadIdx.x & 63);
+  float* at = lds + ((wave_id() % QW) * DT * 16) * 64 + (threadIdx.x & 63);
 #pragma unroll
   for (int i = 0; i < DT; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) at[(i * 16 + r) * 64] = v[i][r];
 }
-template <int DT>
+template <int QW, int DT>
 __device__ __forceinline__ void ja_take(const float* lds, f32x16 (&v)[DT], float mine = 1.f, float its = 1.f) {
-  const float* at = lds + ((wave_id() & 3) * DT * 16) * 64 + (threadIdx.x & 63);
+  const float* at = lds + ((wave_id() % QW) * DT * 16) * 64 + (threadIdx.x & 63);
 #pragma unroll
   for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -383,6 +389,11 @@ __device__ __forceinline__ float half_sum(float v) {
 template <typename T, int DP>
 constexpr bool ja_keep = sizeof(T) == 2 || DP <= 128;
 
+// Whether there are at most two tiles of 128 rows for each CU: two wave sets then share a
+// workgroup's tiles.
+inline bool jagged_few(const JaggedAttnArgs& a, int heads) {
+  return (a.rows / 128 + a.B) * heads <= 2 * device_cus();
+}
 // Checks the sizes and fills in the rest of the arguments.
 int jagged_attn_check(const char* what, JaggedAttnArgs& a, int H, int bf16);
 

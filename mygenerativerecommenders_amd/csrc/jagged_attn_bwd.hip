@@ -16,13 +16,13 @@
 namespace gr {
 
 // dQ: one workgroup per 128 query rows and head, a wave per 32 rows, tiles of BN keys.
-template <typename T, int DP, int BN, int BYTES, int SETS>
-__global__ __launch_bounds__(256 * SETS) void jagged_attn_dq_kernel(JaggedAttnArgs a) {
+template <typename T, int DP, int BN, int BYTES, int QW, int SETS>
+__global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dq_kernel(JaggedAttnArgs a) {
   using F = JaFrag<T>;
   using Tile = JaTile<T, DP>;
-  constexpr int BM = 128, NB = BN / 32, DT = DP / 32, TILE = Tile::size(BN);
+  constexpr int BM = 32 * QW, NB = BN / 32, DT = DP / 32, TILE = Tile::size(BN);
   __shared__ u32x4_t lds[SETS * 4 * TILE];
-  static_assert(SETS == 1 || sizeof(lds) >= 4 * DT * 16 * 256, "a set's sums fit");
+  static_assert(SETS == 1 || sizeof(lds) >= QW * DT * 16 * 256, "a set's sums fit");
   const JaggedWork wk = jagged_work(a, blockIdx.x);
   const int head = wk.hk * a.group + wk.g, H = a.Hkv * a.group;
   const JaggedTile t = jagged_tile<BM>(a.offsets, a.B, a.rows, a.slots - 1 - wk.slot);
@@ -33,17 +33,17 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_dq_kernel(JaggedAttnAr
     return;
   }
   const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5;
-  const int set = SETS > 1 ? wave >> 2 : 0;  // takes tiles set, set + SETS, ..
+  const int set = SETS > 1 ? wave / QW : 0;  // takes tiles set, set + SETS, ..
   u32x4_t *lk = lds + set * 4 * TILE, *lv = lk + 2 * TILE;
-  const int q0 = t.r0 + 32 * (wave & 3), qi = q0 + (lane & 31);
+  const int q0 = t.r0 + 32 * (wave % QW), qi = q0 + (lane & 31);
   const bool ok = qi < t.len;
   const T* kb = (const T*)a.k + t.s0 * a.ld_k + wk.hk * a.hs_k;
   const T* vb = (const T*)a.v + t.s0 * a.ld_v + wk.hk * a.hs_v;
   const int keys = a.causal ? min(t.len, t.r0 + BM) : t.len;
   const int first = set * BN, step = SETS * BN;
   auto load = [&](int k0, int buf) {
-    ja_stage<T, DP, BN, BYTES>(kb, a.ld_k, k0, t.len, a.d, lk + buf);
-    ja_stage<T, DP, BN, BYTES>(vb, a.ld_v, k0, t.len, a.dv, lv + buf);
+    ja_stage<T, DP, BN, BYTES, QW>(kb, a.ld_k, k0, t.len, a.d, lk + buf);
+    ja_stage<T, DP, BN, BYTES, QW>(vb, a.ld_v, k0, t.len, a.dv, lv + buf);
   };
   if (first < keys) load(first, 0);
   JaRows<T, DP, ja_keep<T, DP>> q, go;
@@ -97,10 +97,10 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_dq_kernel(JaggedAttnAr
   }
   if constexpr (SETS > 1) {
     float* sums = reinterpret_cast<float*>(lds);
-    if (set) ja_give(sums, acc);
+    if (set) ja_give<QW>(sums, acc);
     __syncthreads();
     if (set) return;
-    ja_take(sums, acc);
+    ja_take<QW>(sums, acc);
   }
   T* row = dq + (int64_t)(ok ? qi - t.r0 : 0) * H * a.d;
 #pragma unroll
@@ -111,14 +111,14 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_dq_kernel(JaggedAttnAr
 // rows of each query head of the group in turn.  WANT: 1 = dV, 2 = dK, 3 = both in one launch;
 // heads wider than 128 take a launch for each, as both results' accumulators and the
 // keys' fragments do not fit the registers together.
-template <typename T, int DP, int BQ, int WANT, int BYTES, int SETS>
-__global__ __launch_bounds__(256 * SETS) void jagged_attn_dkv_kernel(JaggedAttnArgs a) {
+template <typename T, int DP, int BQ, int WANT, int BYTES, int QW, int SETS>
+__global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dkv_kernel(JaggedAttnArgs a) {
   using F = JaFrag<T>;
   using Tile = JaTile<T, DP>;
-  constexpr int BM = 128, NB = BQ / 32, DT = DP / 32, TILE = Tile::size(BQ);
+  constexpr int BM = 32 * QW, NB = BQ / 32, DT = DP / 32, TILE = Tile::size(BQ);
   __shared__ u32x4_t lds[SETS * 4 * TILE];
   __shared__ __attribute__((aligned(16))) float lsum[SETS * 4 * BQ];
-  static_assert(SETS == 1 || sizeof(lds) >= 4 * DT * 16 * 256, "a set's sums fit");
+  static_assert(SETS == 1 || sizeof(lds) >= QW * DT * 16 * 256, "a set's sums fit");
   const JaggedWork wk = jagged_work(a, blockIdx.x);  // group 1: an item per key head
   const int hk = wk.hk, group = a.heads_per_key, H = a.Hkv * group;
   const JaggedTile t = jagged_tile<BM>(a.offsets, a.B, a.rows, wk.slot);
@@ -131,10 +131,10 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_dkv_kernel(JaggedAttnA
     return;
   }
   const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5;
-  const int set = SETS > 1 ? wave >> 2 : 0, tid = threadIdx.x & 255;
+  const int set = SETS > 1 ? wave / QW : 0, tid = threadIdx.x % (64 * QW);
   u32x4_t *lq = lds + set * 4 * TILE, *lg = lq + 2 * TILE;
   float *ll = lsum + set * 4 * BQ, *ld = ll + 2 * BQ;
-  const int k0 = t.r0 + 32 * (wave & 3), ki = k0 + (lane & 31);
+  const int k0 = t.r0 + 32 * (wave % QW), ki = k0 + (lane & 31);
   const bool ok = ki < t.len;
   const int first = a.causal ? t.r0 : 0, per = (t.len - first + BQ - 1) / BQ, n = per * group;
   float rl = 0.f, rd = 0.f;
@@ -148,8 +148,8 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_dkv_kernel(JaggedAttnA
   };
   if (set) next();  // a set takes every other tile
   auto load = [&](int buf) {
-    ja_stage<T, DP, BQ, BYTES>((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, a.ld_q, r0, t.len, a.d, lq + buf * TILE);
-    ja_stage<T, DP, BQ, BYTES>((const T*)a.dout + (t.s0 * H + head) * a.dv, (int64_t)H * a.dv, r0, t.len, a.dv,
+    ja_stage<T, DP, BQ, BYTES, QW>((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, a.ld_q, r0, t.len, a.d, lq + buf * TILE);
+    ja_stage<T, DP, BQ, BYTES, QW>((const T*)a.dout + (t.s0 * H + head) * a.dv, (int64_t)H * a.dv, r0, t.len, a.dv,
                                lg + buf * TILE);
     if (tid < BQ) {
       const int r = r0 + tid;
@@ -220,15 +220,15 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_dkv_kernel(JaggedAttnA
   if constexpr (SETS > 1) {
     float* sums = reinterpret_cast<float*>(lds);
     if (WANT & 1) {
-      if (set) ja_give(sums, av);
+      if (set) ja_give<QW>(sums, av);
       __syncthreads();
-      if (!set) ja_take(sums, av);
+      if (!set) ja_take<QW>(sums, av);
       if (WANT & 2) __syncthreads();
     }
     if (WANT & 2) {
-      if (set) ja_give(sums, ak);
+      if (set) ja_give<QW>(sums, ak);
       __syncthreads();
-      if (!set) ja_take(sums, ak);
+      if (!set) ja_take<QW>(sums, ak);
     }
     if (set) return;
   }
@@ -241,45 +241,61 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_dkv_kernel(JaggedAttnA
   }
 }
 
-template <typename T, int DP, int BN, int BQ, int BYTES>
-static void bwd_launch(JaggedAttnArgs a, hipStream_t st) {
-  const dim3 gq((unsigned)(a.slots * a.Hkv * a.group)), gk((unsigned)(a.slots * a.Hkv)), one(256), two(512);
-  // two waves a SIMD leave 256 registers: that does for widths of 128 (query pass, bf16) or 64
-  bool done = false;
-  if constexpr (DP * sizeof(T) <= 256) {
-    if (a.sets == 2) {
-      hipLaunchKernelGGL((jagged_attn_dq_kernel<T, DP, BN, BYTES, 2>), gq, two, 0, st, a);
-      done = true;
-    }
-  }
-  if (!done) hipLaunchKernelGGL((jagged_attn_dq_kernel<T, DP, BN, BYTES, 1>), gq, one, 0, st, a);
+template <typename T, int DP, int BN, int BYTES, int QW, int SETS>
+static void dq_run(JaggedAttnArgs a, hipStream_t st) {
+  a.slots = jagged_slots(a.rows, a.B, 32 * QW);
+  hipLaunchKernelGGL((jagged_attn_dq_kernel<T, DP, BN, BYTES, QW, SETS>), dim3((unsigned)(a.slots * a.Hkv * a.group)),
+                     dim3(64 * QW * SETS), 0, st, a);
+}
+template <typename T, int DP, int BQ, int WANT, int BYTES, int QW, int SETS>
+static void dkv_run(JaggedAttnArgs a, hipStream_t st) {
+  a.slots = jagged_slots(a.rows, a.B, 32 * QW);
   a.heads_per_key = a.group;
   a.group = 1;
-  if constexpr (DP == 64) {
-    if (a.sets_k == 2) {
-      hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, 3, BYTES, 2>), gk, two, 0, st, a);
-      return;
+  hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, WANT, BYTES, QW, SETS>), dim3((unsigned)(a.slots * a.Hkv)),
+                     dim3(64 * QW * SETS), 0, st, a);
+}
+template <typename T, int DP, int BYTES>
+static void bwd_shape(const JaggedAttnArgs& a, hipStream_t st) {
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (DP <= 128) {
+      dq_run<T, DP, 32, BYTES, 2, 2>(a, st);
+      dkv_run<T, DP, 32, 3, BYTES, 2, 2>(a, st);
+    } else {
+      dq_run<T, DP, 32, BYTES, 4, 1>(a, st);
+      dkv_run<T, DP, 32, 1, BYTES, 4, 1>(a, st);
+      dkv_run<T, DP, 32, 2, BYTES, 4, 1>(a, st);
     }
-  }
-  if constexpr (DP <= 128) {
-    hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, 3, BYTES, 1>), gk, one, 0, st, a);
+  } else if constexpr (DP == 64) {
+    if (jagged_few(a, a.Hkv * a.group))
+      dq_run<T, DP, 64, BYTES, 4, 2>(a, st);
+    else
+      dq_run<T, DP, 64, BYTES, 4, 1>(a, st);
+    if (jagged_few(a, a.Hkv))
+      dkv_run<T, DP, 64, 3, BYTES, 4, 2>(a, st);
+    else
+      dkv_run<T, DP, 64, 3, BYTES, 4, 1>(a, st);
+  } else if constexpr (DP == 128) {
+    if (jagged_few(a, a.Hkv * a.group))
+      dq_run<T, DP, 32, BYTES, 4, 2>(a, st);
+    else
+      dq_run<T, DP, 32, BYTES, 4, 1>(a, st);
+    dkv_run<T, DP, 32, 3, BYTES, 4, 1>(a, st);
   } else {
-    hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, 1, BYTES, 1>), gk, one, 0, st, a);
-    hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, 2, BYTES, 1>), gk, one, 0, st, a);
+    dq_run<T, DP, 32, BYTES, 4, 1>(a, st);
+    dkv_run<T, DP, 32, 1, BYTES, 4, 1>(a, st);
+    dkv_run<T, DP, 32, 2, BYTES, 4, 1>(a, st);
   }
 }
 template <typename T, int BYTES>
-static void bwd_width(JaggedAttnArgs a, hipStream_t st) {
+static void bwd_width(const JaggedAttnArgs& a, hipStream_t st) {
   const int w = a.d > a.dv ? a.d : a.dv;
-  constexpr int BN = sizeof(T) == 2 ? 64 : 32;
-  a.slots = jagged_slots(a.rows, a.B, 128);
-  a.sets_k = (a.rows / 128 + a.B) * a.Hkv <= 2 * device_cus() ? 2 : 1;
   if (w <= 64)
-    bwd_launch<T, 64, BN, BN, BYTES>(a, st);
+    bwd_shape<T, 64, BYTES>(a, st);
   else if (w <= 128)
-    bwd_launch<T, 128, 32, 32, BYTES>(a, st);
+    bwd_shape<T, 128, BYTES>(a, st);
   else
-    bwd_launch<T, 256, 32, 32, BYTES>(a, st);
+    bwd_shape<T, 256, BYTES>(a, st);
 }
 template <typename T>
 static void bwd_any(const JaggedAttnArgs& a, hipStream_t st) {

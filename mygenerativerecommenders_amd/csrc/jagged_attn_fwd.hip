@@ -15,13 +15,13 @@
 
 namespace gr {
 
-template <typename T, int DP, int BN, int BYTES, int SETS>
-__global__ __launch_bounds__(256 * SETS) void jagged_attn_fwd_kernel(JaggedAttnArgs a) {
+template <typename T, int DP, int BN, int BYTES, int QW, int SETS>
+__global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedAttnArgs a) {
   using F = JaFrag<T>;
   using Tile = JaTile<T, DP>;
-  constexpr int BM = 128, NB = BN / 32, DT = DP / 32, TILE = Tile::size(BN);
+  constexpr int BM = 32 * QW, NB = BN / 32, DT = DP / 32, TILE = Tile::size(BN);
   __shared__ u32x4_t lds[SETS * 4 * TILE];
-  static_assert(SETS == 1 || sizeof(lds) >= (4 * DT * 16 + 8) * 256, "a set's sums fit");
+  static_assert(SETS == 1 || sizeof(lds) >= (QW * DT * 16 + 2 * QW) * 256, "a set's sums fit");
   const JaggedWork wk = jagged_work(a, blockIdx.x);
   const int head = wk.hk * a.group + wk.g, H = a.Hkv * a.group;
   // later tiles of a causal sequence have more keys: they go first
@@ -32,16 +32,16 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_fwd_kernel(JaggedAttnA
     return;
   }
   const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5;
-  const int set = SETS > 1 ? wave >> 2 : 0;  // takes tiles set, set + SETS, ..
+  const int set = SETS > 1 ? wave / QW : 0;  // takes tiles set, set + SETS, ..
   u32x4_t *lk = lds + set * 4 * TILE, *lv = lk + 2 * TILE;
-  const int q0 = t.r0 + 32 * (wave & 3), qi = q0 + (lane & 31);
+  const int q0 = t.r0 + 32 * (wave % QW), qi = q0 + (lane & 31);
   const T* kb = (const T*)a.k + t.s0 * a.ld_k + wk.hk * a.hs_k;
   const T* vb = (const T*)a.v + t.s0 * a.ld_v + wk.hk * a.hs_v;
   const int keys = a.causal ? min(t.len, t.r0 + BM) : t.len;
   const int first = set * BN, step = SETS * BN;
   auto load = [&](int k0, int buf) {
-    ja_stage<T, DP, BN, BYTES>(kb, a.ld_k, k0, t.len, a.d, lk + buf);
-    ja_stage<T, DP, BN, BYTES>(vb, a.ld_v, k0, t.len, a.dv, lv + buf);
+    ja_stage<T, DP, BN, BYTES, QW>(kb, a.ld_k, k0, t.len, a.d, lk + buf);
+    ja_stage<T, DP, BN, BYTES, QW>(vb, a.ld_v, k0, t.len, a.dv, lv + buf);
   };
   if (first < keys) load(first, 0);
   JaRows<T, DP, ja_keep<T, DP>> q;
@@ -98,9 +98,9 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_fwd_kernel(JaggedAttnA
   }
   l = half_sum(l);
   if constexpr (SETS > 1) {
-    float *sums = reinterpret_cast<float*>(lds), *ml = sums + 4 * DT * 16 * 64 + (wave & 3) * 128 + lane;
+    float *sums = reinterpret_cast<float*>(lds), *ml = sums + QW * DT * 16 * 64 + (wave % QW) * 128 + lane;
     if (set) {
-      ja_give(sums, o);
+      ja_give<QW>(sums, o);
       ml[0] = m;
       ml[64] = l;
     }
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(256 * SETS) void jagged_attn_fwd_kernel(JaggedAttnA
     if (set) return;
     const float top = fmaxf(m, ml[0]), f = __builtin_amdgcn_exp2f((m - top) * a.scale_l2),
                 g = __builtin_amdgcn_exp2f((ml[0] - top) * a.scale_l2);
-    ja_take(sums, o, f, g);
+    ja_take<QW>(sums, o, f, g);
     l = l * f + ml[64] * g;
     m = top;
   }
@@ -138,37 +138,44 @@ int jagged_attn_check(const char* what, JaggedAttnArgs& a, int H, int bf16) {
              "%s: row strides outside [0, 2^22)", what);
   a.wide = at % 16 == 0 && steps % least == 0;
   a.group = H / a.Hkv;
-  const int64_t tiles = (a.rows / 128 + a.B) * H;
-  a.sets = tiles <= 2 * device_cus() ? 2 : 1;
-  return 0;
+    return 0;
 }
 
-template <typename T, int DP, int BN, int BYTES>
-static void fwd_sets(const JaggedAttnArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)(a.slots * a.Hkv * a.group));
-  // two waves a SIMD leave 256 registers: widths of 128 (fp32: 64) at most
-  if constexpr (DP * sizeof(T) <= 256) {
-    if (a.sets == 2) {
-      hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, DP, BN, BYTES, 2>), grid, dim3(512), 0, st, a);
-      return;
-    }
+template <typename T, int DP, int BN, int BYTES, int QW, int SETS>
+static void fwd_run(JaggedAttnArgs a, hipStream_t st) {
+  a.slots = jagged_slots(a.rows, a.B, 32 * QW);
+  hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, DP, BN, BYTES, QW, SETS>), dim3((unsigned)(a.slots * a.Hkv * a.group)),
+                     dim3(64 * QW * SETS), 0, st, a);
+}
+template <typename T, int DP, int BYTES>
+static void fwd_shape(const JaggedAttnArgs& a, hipStream_t st) {
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (DP <= 128)
+      fwd_run<T, DP, 32, BYTES, 2, 2>(a, st);
+    else
+      fwd_run<T, DP, 32, BYTES, 4, 1>(a, st);
+  } else if constexpr (DP <= 128) {
+    if (jagged_few(a, a.Hkv * a.group))
+      fwd_run<T, DP, 64, BYTES, 4, 2>(a, st);
+    else
+      fwd_run<T, DP, 64, BYTES, 4, 1>(a, st);
+  } else {
+    fwd_run<T, DP, 32, BYTES, 4, 1>(a, st);
   }
-  hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, DP, BN, BYTES, 1>), grid, dim3(256), 0, st, a);
 }
-template <typename T, int DP, int BN>
-static void fwd_launch(const JaggedAttnArgs& a, hipStream_t st) {
-  a.wide ? fwd_sets<T, DP, BN, 16>(a, st) : fwd_sets<T, DP, BN, 4>(a, st);
-}
-template <typename T>
+template <typename T, int BYTES>
 static void fwd_width(const JaggedAttnArgs& a, hipStream_t st) {
   const int w = a.d > a.dv ? a.d : a.dv;
-  constexpr int BN = sizeof(T) == 2 ? 64 : 32;
   if (w <= 64)
-    fwd_launch<T, 64, BN>(a, st);
+    fwd_shape<T, 64, BYTES>(a, st);
   else if (w <= 128)
-    fwd_launch<T, 128, BN>(a, st);
+    fwd_shape<T, 128, BYTES>(a, st);
   else
-    fwd_launch<T, 256, 32>(a, st);
+    fwd_shape<T, 256, BYTES>(a, st);
+}
+template <typename T>
+static void fwd_any(const JaggedAttnArgs& a, hipStream_t st) {
+  a.wide ? fwd_width<T, 16>(a, st) : fwd_width<T, 4>(a, st);
 }
 
 }  // namespace gr
@@ -187,9 +194,8 @@ extern "C" int gr_jagged_attn_fwd(const void* q, int64_t ld_q, int64_t hs_q, con
   a.out = out; a.out_low = out_low; a.lse = lse;
   if (gr::jagged_attn_check("gr_jagged_attn_fwd", a, H, bf16)) return 1;
   if (rows == 0) return 0;
-  a.slots = gr::jagged_slots(rows, B, 128);
   const hipStream_t st = (hipStream_t)stream;
-  GR_TIMED("jagged_attn_fwd", st, bf16 ? gr::fwd_width<__bf16>(a, st) : gr::fwd_width<float>(a, st));
+  GR_TIMED("jagged_attn_fwd", st, bf16 ? gr::fwd_any<__bf16>(a, st) : gr::fwd_any<float>(a, st));
   GR_LAUNCH_CHECK("gr_jagged_attn_fwd");
   return 0;
 }
