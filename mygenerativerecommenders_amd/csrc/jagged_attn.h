@@ -79,20 +79,46 @@ inline int64_t jagged_slots(int64_t rows, int B, int bm) { return rows / bm + B 
 __device__ __forceinline__ int64_t ja_clamp(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
 template <int BM>
 __device__ __forceinline__ JaggedTile jagged_tile(const int64_t* offsets, int B, int64_t rows, int64_t slot) {
-  int lo = 0, hi = B + 1;
+  int lo = 0;
   const int lane = threadIdx.x & 63;
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 63) >> 6;
-    const int i = lo + lane * step;
-    const bool le = i < hi && ja_clamp(offsets[i < hi ? i : B], 0, rows) / BM + i <= slot;
-    const int c = __popcll(__ballot(le));
-    lo += (c > 0 ? c - 1 : 0) * step;
-    hi = hi < lo + step ? hi : lo + step;
-  }
   JaggedTile t;
-  t.s0 = ja_clamp(offsets[lo], 0, rows);
+  int64_t end;
+  if (B < 256) {  // all of them at once: one round trip to memory
+    int64_t at[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (64 * j <= B) at[j] = ja_clamp(offsets[min(64 * j + lane, B)], 0, rows);
+    lo = -1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (64 * j <= B) lo += __popcll(__ballot(64 * j + lane <= B && at[j] / BM + 64 * j + lane <= slot));
+    lo = lo < 0 ? 0 : lo;
+    auto value = [&](int i) {
+      int64_t v = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (64 * j <= B && i >> 6 == j) v = at[j];
+      return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, i & 63) |
+             (int64_t)__builtin_amdgcn_readlane((int)(v >> 32), i & 63) << 32;
+    };
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    t.s0 = value(lo);
+    end = lo == B ? rows : value(lo + 1);
+  } else {
+    int hi = B + 1;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 63) >> 6;
+      const int i = lo + lane * step;
+      const bool le = i < hi && ja_clamp(offsets[i < hi ? i : B], 0, rows) / BM + i <= slot;
+      const int c = __popcll(__ballot(le));
+      lo += (c > 0 ? c - 1 : 0) * step;
+      hi = hi < lo + step ? hi : lo + step;
+    }
+    t.s0 = ja_clamp(offsets[lo], 0, rows);
+    end = lo == B ? rows : ja_clamp(offsets[lo + 1], 0, rows);
+  }
   t.tail = lo == B;
-  const int64_t end = t.tail ? rows : ja_clamp(offsets[lo + 1], t.s0, rows);
+  if (end < t.s0) end = t.s0;
   const int64_t r0 = (slot - lo - t.s0 / BM) * BM;
   t.len = r0 >= 0 && r0 < end - t.s0 ? (int)(end - t.s0) : 0;
   t.r0 = (int)r0;
@@ -102,7 +128,7 @@ __device__ __forceinline__ JaggedTile jagged_tile(const int64_t* offsets, int B,
 // 16 bytes of a row from column c, for rows of `d` >= 16 bytes of any alignment, in two steps
 // so that the first can stay in flight: ja_load16 reads inside the row always (the vector
 // that would cross its end is read up against it), ja_fix16 moves such a vector's elements
-// down and clears what lies past column d, or all of it where `ok` is false.
+// down and clears what lies past column d.
 template <typename T>
 __device__ __forceinline__ u32x4_t ja_load16(const T* row, int c, int d) {
   constexpr int V = 16 / sizeof(T);
@@ -112,7 +138,7 @@ __device__ __forceinline__ u32x4_t ja_load16(const T* row, int c, int d) {
   return reinterpret_cast<const P*>(row + min(c, d - V))->v;
 }
 template <typename T>
-__device__ __forceinline__ u32x4_t ja_fix16(u32x4_t x, int c, int d, bool ok) {
+__device__ __forceinline__ u32x4_t ja_fix16(u32x4_t x, int c, int d) {
   constexpr int V = 16 / sizeof(T);
   if (d % V != 0) {  // uniform
     unsigned __int128 w = __builtin_bit_cast(unsigned __int128, x);
@@ -120,7 +146,7 @@ __device__ __forceinline__ u32x4_t ja_fix16(u32x4_t x, int c, int d, bool ok) {
     x = __builtin_bit_cast(u32x4_t, w);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = ok && c < d ? x[i] : 0u;
+  for (int i = 0; i < 4; ++i) x[i] = c < d ? x[i] : 0u;
   return x;
 }
 
@@ -259,24 +285,24 @@ struct JaFrag<float> {
 };
 
 // A wave's 32 rows of an operand as fragments: in registers, or (where the registers of the
-// widest fp32 heads do not hold them) read again from cache at every use.
+// widest fp32 heads do not hold them) read again from cache at every use.  Rows past the end
+// repeat the last one: what comes of them is not stored.
 template <typename T, int DP, bool KEEP>
 struct JaRows {
   static constexpr int K = JaFrag<T>::K, KS = DP / K;
   u32x4_t x[KEEP ? KS : 1];
   const T* row;
   int d;
-  bool ok;
   __device__ __forceinline__ void init(const T* base, int64_t ld, int r0, int len, int width) {
     const int lane = threadIdx.x & 63, r = r0 + (lane & 31);
-    ok = r < len;
     row = base + (int64_t)min(r, len - 1) * ld;
     d = width;
     if constexpr (KEEP) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) x[s] = ja_load16<T>(row, col(s), d);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) x[s] = ja_fix16<T>(x[s], col(s), d, ok);
+      for (int s = 0; s < KS; ++s)
+        if (K * s + K > d) x[s] = ja_fix16<T>(x[s], col(s), d);
     }
   }
   static __device__ __forceinline__ int col(int s) { return K * s + K / 2 * ((threadIdx.x & 63) >> 5); }
@@ -286,7 +312,8 @@ struct JaRows {
   }
   __device__ __forceinline__ u32x4_t at(int s) const {
     if constexpr (KEEP) return x[s];
-    return ja_fix16<T>(ja_load16<T>(row, col(s), d), col(s), d, ok);
+    const u32x4_t v = ja_load16<T>(row, col(s), d);
+    return K * s + K > d ? ja_fix16<T>(v, col(s), d) : v;
   }
 };
 

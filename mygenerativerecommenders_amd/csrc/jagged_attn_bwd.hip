@@ -272,7 +272,7 @@ static void bwd_shape(const JaggedAttnArgs& a, hipStream_t st) {
     else
       dq_run<T, DP, 64, BYTES, 4, 1>(a, st);
     if (jagged_few(a, a.Hkv))
-      dkv_run<T, DP, 64, 3, BYTES, 4, 2>(a, st);
+      dkv_run<T, DP, 32, 3, BYTES, 2, 2>(a, st);
     else
       dkv_run<T, DP, 64, 3, BYTES, 4, 1>(a, st);
   } else if constexpr (DP == 128) {
@@ -280,11 +280,11 @@ static void bwd_shape(const JaggedAttnArgs& a, hipStream_t st) {
       dq_run<T, DP, 32, BYTES, 4, 2>(a, st);
     else
       dq_run<T, DP, 32, BYTES, 4, 1>(a, st);
-    dkv_run<T, DP, 32, 3, BYTES, 4, 1>(a, st);
+    dkv_run<T, DP, 32, 3, BYTES, 2, 2>(a, st);
   } else {
-    dq_run<T, DP, 32, BYTES, 4, 1>(a, st);
-    dkv_run<T, DP, 32, 1, BYTES, 4, 1>(a, st);
-    dkv_run<T, DP, 32, 2, BYTES, 4, 1>(a, st);
+    dq_run<T, DP, 32, BYTES, 2, 2>(a, st);
+    dkv_run<T, DP, 32, 1, BYTES, 2, 2>(a, st);
+    dkv_run<T, DP, 32, 2, BYTES, 2, 2>(a, st);
   }
 }
 template <typename T, int BYTES>

@@ -160,7 +160,7 @@ static void fwd_shape(const JaggedAttnArgs& a, hipStream_t st) {
     else
       fwd_run<T, DP, 64, BYTES, 4, 1>(a, st);
   } else {
-    fwd_run<T, DP, 32, BYTES, 4, 1>(a, st);
+    fwd_run<T, DP, 32, BYTES, 2, 2>(a, st);
   }
 }
 template <typename T, int BYTES>
