@@ -67,26 +67,30 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedA
           for (int r = 0; r < 16; ++r)
             if (k0 + 32 * b + (r & 3) + 8 * (r >> 2) + 4 * half > last) s[b][r] = -INFINITY;
       }
-      float top = m;
+      float top = -INFINITY;
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
       top = half_max(top);
-      const float f = __builtin_amdgcn_exp2f((m - top) * a.scale_l2);
-      m = top;
+      // Sums are relative to m, which follows the maximum only once that is 2^8 ahead: what is
+      // summed stays below 2^8 times the rows, and the rescaling is rare.
+      if (__builtin_expect(__any((top - m) * a.scale_l2 > 8.f), 0)) {
+        top = fmaxf(top, m);
+        const float f = __builtin_amdgcn_exp2f((m - top) * a.scale_l2);
+        m = top;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) o[i] *= f;
+      }
       const float mc = m * a.scale_l2;
-      float sum = 0.f;
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           s[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], a.scale_l2, -mc));
-          sum += s[b][r];
+          l += s[b][r];
         }
-      l = l * f + sum;
-#pragma unroll
-      for (int i = 0; i < DT; ++i) o[i] *= f;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const typename F::Rows p(s[b]);
