@@ -8,6 +8,8 @@
 // (r & 3) + 8 (r >> 2) + 4 h, and the other operand is read from LDS in that row order.
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
 #include "mfma32.h"
 
@@ -41,34 +43,44 @@ struct JaggedAttnArgs {
   int heads_per_key; // the backward's key pass: `group`, where that is 1 for its grid
 };
 
-// Work item of a workgroup.  Workgroups i, i + 8, .. land on one XCD: each XCD takes a
-// contiguous eighth of the items, heads of a group next to each other, so that one L2 serves
-// the tiles and heads that read the same keys and values.  Of a causal sequence's tiles the
-// heavy come first; every other round over the XCD's 32 CUs runs backwards, so that a CU that
-// got a heavy tile gets a light one next.
+// Work item of a workgroup: slot, key head, and query head of its group.  Workgroups i, i + 8, ..
+// land on one XCD: the heads of a group follow each other there, so that its L2 serves them the
+// same keys and values.
 struct JaggedWork {
   int hk, g;
-  int64_t slot;
+  int64_t slot;  // >= slots: nothing
 };
+inline int64_t jagged_grid(int64_t slots, int Hkv, int group) { return (slots * Hkv + 7) / 8 * 8 * group; }
 __device__ __forceinline__ JaggedWork jagged_work(const JaggedAttnArgs& a, unsigned id) {
-  const unsigned n = gridDim.x, per = n / 8, more = n % 8, x = id % 8;
-  unsigned j = id / 8;
-  const unsigned mine = per + (x < more), round = j / 32 * 32;
-  if (j & 32) j = round + (mine - round < 32 ? mine - round : 32) - 1 - (j - round);
-  const unsigned w = x * per + (x < more ? x : more) + j;
-  const unsigned slots = (unsigned)a.slots, group = (unsigned)a.group;
+  const unsigned group = (unsigned)a.group, j = id / 8, u = j / group * 8 + id % 8;
   JaggedWork k;
-  k.g = (int)(w % group);
-  k.slot = w / group % slots;
-  k.hk = (int)(w / group / slots);
+  k.g = (int)(j % group);
+  k.slot = u / (unsigned)a.Hkv;
+  k.hk = (int)(u % (unsigned)a.Hkv);
   return k;
 }
 
-// Tile `slot` of the jagged rows in tiles of BM rows that never cross a sequence: sequence b
-// owns the slots from offsets[b] / BM + b on, which always leaves it enough of them, so
-// neither the longest length nor a prefix of tile counts is needed on the host.  The rows
-// past the last sequence are tiled as one more (`tail`).  A search over the offsets, 64 at a
-// time.  Offsets outside the rows are clamped.
+// Sum over the wave, in every lane.
+__device__ __forceinline__ int wave_isum(int v) {
+  auto mov = [](int x, auto ctrl) { return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, 0xF, 0xF, true); };
+  v += mov(v, std::integral_constant<int, 0xB1>{});   // quad_perm [1,0,3,2]
+  v += mov(v, std::integral_constant<int, 0x4E>{});   // quad_perm [2,3,0,1]
+  v += mov(v, std::integral_constant<int, 0x141>{});  // row_half_mirror
+  v += mov(v, std::integral_constant<int, 0x140>{});  // row_mirror
+  return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) +
+         __builtin_amdgcn_readlane(v, 48);
+}
+
+// Tile `slot` of the jagged rows in tiles of BM rows that never cross a sequence; the rows past
+// the last sequence are tiled as one more (`tail`).  The host knows neither lengths nor tile
+// counts, only that rows / BM + B + 1 slots are enough.  Offsets are clamped to the rows.
+//
+// Up to 255 sequences the wave holds them all, and slots run from the heavy tiles to the light
+// ones: level n of a sequence is the tile that meets n tiles of a causal sequence's other side
+// (`keys`: the key rows' pass, where that is the n-th from the end), slots go down the levels
+// and through the sequences that reach them.  Workgroups start in that order, so the longest
+// do not run alone at the end.  With more sequences, sequence b owns the slots from
+// offsets[b] / BM + b on, found by a search over the offsets, 64 at a time.
 struct JaggedTile {
   int64_t s0;  // first row of the sequence
   int len;     // its length (0: the slot holds no tile)
@@ -77,48 +89,79 @@ struct JaggedTile {
 };
 inline int64_t jagged_slots(int64_t rows, int B, int bm) { return rows / bm + B + 1; }
 __device__ __forceinline__ int64_t ja_clamp(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
-template <int BM>
+template <int BM, bool KEYS>
 __device__ __forceinline__ JaggedTile jagged_tile(const int64_t* offsets, int B, int64_t rows, int64_t slot) {
-  int lo = 0;
   const int lane = threadIdx.x & 63;
   JaggedTile t;
-  int64_t end;
-  if (B < 256) {  // all of them at once: one round trip to memory
-    int64_t at[4];
+  t.tail = false;
+  if (B < 256) {
+    int first[4], tiles[4], lens[4], total = 0;  // rows < 2^31
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (64 * j <= B) at[j] = ja_clamp(offsets[min(64 * j + lane, B)], 0, rows);
-    lo = -1;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (64 * j <= B) lo += __popcll(__ballot(64 * j + lane <= B && at[j] / BM + 64 * j + lane <= slot));
-    lo = lo < 0 ? 0 : lo;
-    auto value = [&](int i) {
-      int64_t v = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (64 * j <= B && i >> 6 == j) v = at[j];
-      return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, i & 63) |
-             (int64_t)__builtin_amdgcn_readlane((int)(v >> 32), i & 63) << 32;
-    };
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    t.s0 = value(lo);
-    end = lo == B ? rows : value(lo + 1);
-  } else {
-    int hi = B + 1;
-    while (hi - lo > 1) {
-      const int step = (hi - lo + 63) >> 6;
-      const int i = lo + lane * step;
-      const bool le = i < hi && ja_clamp(offsets[i < hi ? i : B], 0, rows) / BM + i <= slot;
-      const int c = __popcll(__ballot(le));
-      lo += (c > 0 ? c - 1 : 0) * step;
-      hi = hi < lo + step ? hi : lo + step;
+    for (int j = 0; j < 4; ++j) {
+      first[j] = tiles[j] = lens[j] = 0;
+      if (64 * j < B) {  // uniform
+        const int i = 64 * j + lane;
+        const int64_t lo = ja_clamp(offsets[i < B ? i : B], 0, rows), hi = ja_clamp(offsets[i < B ? i + 1 : B], lo, rows);
+        first[j] = (int)lo;
+        lens[j] = i < B ? (int)(hi - lo) : 0;
+        tiles[j] = (lens[j] + BM - 1) / BM;
+      }
     }
-    t.s0 = ja_clamp(offsets[lo], 0, rows);
-    end = lo == B ? rows : ja_clamp(offsets[lo + 1], 0, rows);
+    auto above = [&](int n) {  // tiles of level n and more
+      int c = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c += tiles[j] >= n ? tiles[j] - n + 1 : 0;
+      return wave_isum(c);
+    };
+    total = above(1);
+    if (slot >= total) {
+      const int64_t end = ja_clamp(B > 0 ? offsets[B] : 0, 0, rows), r0 = (slot - total) * BM;
+      t.tail = true;
+      t.s0 = end;
+      t.len = r0 < rows - end ? (int)(rows - end) : 0;
+      t.r0 = (int)r0;
+      return t;
+    }
+    int n = 1, more = (int)(rows / BM) + 2, past = 0;  // level n has the slot or is below it
+    while (more - n > 1) {
+      const int mid = (n + more) >> 1, c = above(mid);
+      if (c > slot) {
+        n = mid;
+      } else {
+        more = mid;
+        past = c;
+      }
+    }
+    int k = (int)slot - past;  // the k-th sequence that reaches level n
+    t.s0 = 0;
+    t.len = t.r0 = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const unsigned long long reach = __ballot(tiles[j] >= n);
+      const int c = __popcll(reach);
+      if (k >= 0 && k < c) {  // uniform
+        const bool me = tiles[j] >= n && (int)__popcll(reach & ((1ull << lane) - 1ull)) == k;
+        const int at = __ffsll(__ballot(me)) - 1;
+        t.s0 = __builtin_amdgcn_readlane(first[j], at);
+        t.len = __builtin_amdgcn_readlane(lens[j], at);
+        t.r0 = (KEYS ? __builtin_amdgcn_readlane(tiles[j], at) - n : n - 1) * BM;
+      }
+      k = k < c ? -1 : k - c;
+    }
+    return t;
   }
+  int lo = 0, hi = B + 1;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) >> 6;
+    const int i = lo + lane * step;
+    const bool le = i < hi && ja_clamp(offsets[i < hi ? i : B], 0, rows) / BM + i <= slot;
+    const int c = __popcll(__ballot(le));
+    lo += (c > 0 ? c - 1 : 0) * step;
+    hi = hi < lo + step ? hi : lo + step;
+  }
+  t.s0 = ja_clamp(offsets[lo], 0, rows);
   t.tail = lo == B;
-  if (end < t.s0) end = t.s0;
+  const int64_t end = t.tail ? rows : ja_clamp(offsets[lo + 1], t.s0, rows);
   const int64_t r0 = (slot - lo - t.s0 / BM) * BM;
   t.len = r0 >= 0 && r0 < end - t.s0 ? (int)(end - t.s0) : 0;
   t.r0 = (int)r0;
@@ -178,43 +221,74 @@ struct JaTile {
 // descriptor ends with the sequence's last row, so rows past it come as zeros, and lanes past
 // column d ask for what is out of its range.
 template <typename T, int DP, int R, int BYTES, int QW>
-__device__ __forceinline__ void ja_stage(const T* base, int64_t ld, int r0, int len, int d, u32x4_t* tile) {
+struct JaStage {
   using Tile = JaTile<T, DP>;
-  constexpr int SZ = sizeof(T), PER = 16 / BYTES;             // lanes that share a unit
-  constexpr int N = R * Tile::UNITS * PER / (64 * QW);        // instructions of a wave
+  static constexpr int SZ = sizeof(T), PER = 16 / BYTES;             // lanes that share a unit
+  static constexpr int N = R * Tile::UNITS * PER / (64 * QW);        // instructions of a wave
   // an instruction writes 1 / PER of a kilobyte of the tile; the waves take them in turn, so a
   // wave meets PH different parts of a kilobyte, each with its own columns
-  constexpr int PH = PER > QW ? PER / QW : 1, BLOCKS = QW > PER ? QW / PER : 1;  // kilobytes a turn
+  static constexpr int PH = PER > QW ? PER / QW : 1, BLOCKS = QW > PER ? QW / PER : 1;  // kilobytes a turn
   static_assert(R * Tile::UNITS * PER % (64 * QW) == 0 && Tile::UNITS <= 64, "whole instructions");
-  const int lane = threadIdx.x & 63, w = wave_id() % QW;
-  uint32_t off[PH];
+  uint32_t off[PH], at;  // this wave's place in memory and in the tile at LDS address 0
+  uint64_t p;            // the next tile's first row
+  int64_t left;          // bytes from there to the end of the sequence's last row
+  int row;               // of a row
+  // Rows r0 on of a sequence's `len`, d columns wide.
+  __device__ __forceinline__ void init(const T* base, int64_t ld, int r0, int len, int d) {
+    const int lane = threadIdx.x & 63, w = wave_id() % QW;
+    row = (int)ld * SZ;  // ld < 2^22
 #pragma unroll
-  for (int i = 0; i < PH; ++i) {
-    const int u = (i * QW + w) * 64 / PER + lane / PER, r = u / Tile::UNITS;
-    const int c = (u % Tile::UNITS ^ Tile::swizzle(r)) * Tile::V + lane % PER * (BYTES / SZ);
-    off[i] = c < d ? (uint32_t)(r * (int)ld + c) * SZ : (uint32_t)OOB_OFF;  // ld < 2^22
+    for (int i = 0; i < PH; ++i) {
+      const int u = (i * QW + w) * 64 / PER + lane / PER, r = u / Tile::UNITS;
+      const int c = (u % Tile::UNITS ^ Tile::swizzle(r)) * Tile::V + lane % PER * (BYTES / SZ);
+      off[i] = c < d ? (uint32_t)(r * row + c * SZ) : (uint32_t)OOB_OFF;
+    }
+    at = 1040u * (w / PER) + 1024u / PER * (w % PER);
+    seek(base, r0, len, d);
   }
-  const uint32_t at = __builtin_amdgcn_readfirstlane(
-      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u32x4_t*)tile + 1040u * (w / PER) + 1024u / PER * (w % PER));
-  const uint64_t p = (uint64_t)(base + (int64_t)r0 * ld);
-  const int64_t bytes = ((int64_t)(len - r0 - 1) * ld + d) * SZ;
-  const u32x4_t desc = {(uint32_t)p, (uint32_t)(p >> 32) & 0xFFFFu, (uint32_t)(bytes < 0x7FFFFFFF ? bytes : 0x7FFFFFFF),
-                        0x00020000u};
+  __device__ __forceinline__ void seek(const T* base, int r0, int len, int d) {
+    p = (uint64_t)base + (int64_t)r0 * row;
+    left = (int64_t)(len - r0 - 1) * row + d * SZ;
+  }
+  // The tile at p to LDS, and p on by `rows`.
+  __device__ __forceinline__ void load(uint32_t lds, int rows) {
+    const u32x4_t desc = {(uint32_t)p, (uint32_t)(p >> 32) & 0xFFFFu, (uint32_t)(left < 0x7FFFFFFF ? left : 0x7FFFFFFF),
+                          0x00020000u};
+    const uint32_t base = __builtin_amdgcn_readfirstlane(lds + at);
+    auto to = [&](int i) { return base + 1040u * BLOCKS * (i / PH) + (i % PH) * (1024u / PER * QW); };
+    int turn = BLOCKS * Tile::RPI * row;
+    asm volatile("" : "+s"(turn));  // its multiples are made here, not kept in registers
+    auto from = [&](int i) { return i / PH * turn; };
+    uint32_t keep;  // m0 is saved and put back: the compiler may hold something in it
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    uint32_t keep;
-    const int turn = i / PH;
-    const uint32_t to = at + 1040u * BLOCKS * turn + (i % PH) * (1024u / PER * QW);
-    const int from = BLOCKS * Tile::RPI * SZ * turn * (int)ld;
-    if constexpr (BYTES == 16)
-      asm volatile(
-          "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
-          : "=&s"(keep) : "s"(to), "v"(off[i % PH]), "s"(desc), "s"(from) : "memory");
-    else
-      asm volatile(
-          "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
-          : "=&s"(keep) : "s"(to), "v"(off[i % PH]), "s"(desc), "s"(from) : "memory");
+    for (int i = 0; i < N; i += 2) {
+      if constexpr (N % 2 != 0) {
+        static_assert(N == 1 && BYTES == 16);
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds\n\t"
+                     "s_mov_b32 m0, %0"
+                     : "=&s"(keep) : "s"(to(i)), "v"(off[0]), "s"(desc), "s"(from(i)) : "memory");
+      } else if constexpr (BYTES == 16) {
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds\n\t"
+                     "s_mov_b32 m0, %5\n\ts_nop 0\n\tbuffer_load_dwordx4 %6, %3, %7 offen lds\n\ts_mov_b32 m0, %0"
+                     : "=&s"(keep)
+                     : "s"(to(i)), "v"(off[i % PH]), "s"(desc), "s"(from(i)), "s"(to(i + 1)), "v"(off[(i + 1) % PH]),
+                       "s"(from(i + 1))
+                     : "memory");
+      } else {
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, %4 offen lds\n\t"
+                     "s_mov_b32 m0, %5\n\ts_nop 0\n\tbuffer_load_dword %6, %3, %7 offen lds\n\ts_mov_b32 m0, %0"
+                     : "=&s"(keep)
+                     : "s"(to(i)), "v"(off[i % PH]), "s"(desc), "s"(from(i)), "s"(to(i + 1)), "v"(off[(i + 1) % PH]),
+                       "s"(from(i + 1))
+                     : "memory");
+      }
+    }
+    p += (int64_t)rows * row;
+    left -= (int64_t)rows * row;
   }
+};
+__device__ __forceinline__ uint32_t ja_lds(const u32x4_t* tile) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const u32x4_t*)tile;
 }
 __device__ __forceinline__ void ja_landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 

@@ -24,8 +24,9 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dq_kernel(JaggedAt
   __shared__ u32x4_t lds[SETS * 4 * TILE];
   static_assert(SETS == 1 || sizeof(lds) >= QW * DT * 16 * 256, "a set's sums fit");
   const JaggedWork wk = jagged_work(a, blockIdx.x);
+  if (wk.slot >= a.slots) return;
   const int head = wk.hk * a.group + wk.g, H = a.Hkv * a.group;
-  const JaggedTile t = jagged_tile<BM>(a.offsets, a.B, a.rows, a.slots - 1 - wk.slot);
+  const JaggedTile t = jagged_tile<BM, false>(a.offsets, a.B, a.rows, wk.slot);
   if (t.len == 0) return;
   T* dq = (T*)a.dq + ((t.s0 + t.r0) * H + head) * a.d;
   if (t.tail) {
@@ -41,11 +42,14 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dq_kernel(JaggedAt
   const T* vb = (const T*)a.v + t.s0 * a.ld_v + wk.hk * a.hs_v;
   const int keys = a.causal ? min(t.len, t.r0 + BM) : t.len;
   const int first = set * BN, step = SETS * BN;
-  auto load = [&](int k0, int buf) {
-    ja_stage<T, DP, BN, BYTES, QW>(kb, a.ld_k, k0, t.len, a.d, lk + buf);
-    ja_stage<T, DP, BN, BYTES, QW>(vb, a.ld_v, k0, t.len, a.dv, lv + buf);
+  JaStage<T, DP, BN, BYTES, QW> sk, sv;
+  sk.init(kb, a.ld_k, first, t.len, a.d);
+  sv.init(vb, a.ld_v, first, t.len, a.dv);
+  auto load = [&](int buf) {
+    sk.load(ja_lds(lk + buf), step);
+    sv.load(ja_lds(lv + buf), step);
   };
-  if (first < keys) load(first, 0);
+  if (first < keys) load(0);
   JaRows<T, DP, ja_keep<T, DP>> q, go;
   q.init((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, a.ld_q, q0, t.len, a.d);
   const int64_t out0 = (t.s0 * H + head) * a.dv;
@@ -74,7 +78,7 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dq_kernel(JaggedAt
   for (int i = 0; i < DT; ++i) acc[i] = f16_zero();
   ja_landed();
   for (int k0 = first, buf = 0; k0 - first < keys; k0 += step, buf = TILE - buf) {
-    if (k0 + step < keys) load(k0 + step, TILE - buf);
+    if (k0 + step < keys) load(TILE - buf);
     if (q0 < t.len && k0 < keys && !(a.causal && k0 > q0 + 31)) {
       const bool edge = k0 + BN > t.len || (a.causal && k0 + BN - 1 > q0);
       const int last = a.causal ? min(t.len - 1, qi) : t.len - 1;
@@ -119,9 +123,10 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dkv_kernel(JaggedA
   __shared__ u32x4_t lds[SETS * 4 * TILE];
   __shared__ __attribute__((aligned(16))) float lsum[SETS * 4 * BQ];
   static_assert(SETS == 1 || sizeof(lds) >= QW * DT * 16 * 256, "a set's sums fit");
-  const JaggedWork wk = jagged_work(a, blockIdx.x);  // group 1: an item per key head
+  const JaggedWork wk = jagged_work(a, blockIdx.x);
+  if (wk.slot >= a.slots) return;  // group 1: an item per key head
   const int hk = wk.hk, group = a.heads_per_key, H = a.Hkv * group;
-  const JaggedTile t = jagged_tile<BM>(a.offsets, a.B, a.rows, wk.slot);
+  const JaggedTile t = jagged_tile<BM, true>(a.offsets, a.B, a.rows, wk.slot);
   if (t.len == 0) return;
   T* dk = (T*)a.dk + ((t.s0 + t.r0) * a.Hkv + hk) * a.d;
   T* dv = (T*)a.dvv + ((t.s0 + t.r0) * a.Hkv + hk) * a.dv;
@@ -139,18 +144,26 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dkv_kernel(JaggedA
   const int first = a.causal ? t.r0 : 0, per = (t.len - first + BQ - 1) / BQ, n = per * group;
   float rl = 0.f, rd = 0.f;
   int r0 = first, head = hk * group;  // the tile last loaded: query rows r0 on of a head
+  JaStage<T, DP, BQ, BYTES, QW> sq, sg;
   auto next = [&]() {
     r0 += BQ;
     if (r0 >= t.len) {
       r0 = first;
       ++head;
+      return true;
     }
+    return false;
+  };
+  auto seek = [&]() {
+    sq.seek((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, r0, t.len, a.d);
+    sg.seek((const T*)a.dout + (t.s0 * H + head) * a.dv, r0, t.len, a.dv);
   };
   if (set) next();  // a set takes every other tile
+  sq.init((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, a.ld_q, r0, t.len, a.d);
+  sg.init((const T*)a.dout + (t.s0 * H + head) * a.dv, (int64_t)H * a.dv, r0, t.len, a.dv);
   auto load = [&](int buf) {
-    ja_stage<T, DP, BQ, BYTES, QW>((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, a.ld_q, r0, t.len, a.d, lq + buf * TILE);
-    ja_stage<T, DP, BQ, BYTES, QW>((const T*)a.dout + (t.s0 * H + head) * a.dv, (int64_t)H * a.dv, r0, t.len, a.dv,
-                               lg + buf * TILE);
+    sq.load(ja_lds(lq + buf * TILE), SETS * BQ);
+    sg.load(ja_lds(lg + buf * TILE), SETS * BQ);
     if (tid < BQ) {
       const int r = r0 + tid;
       rl = r < t.len ? a.lse[head * a.rows + t.s0 + r] : INFINITY;  // no probability
@@ -178,8 +191,9 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dkv_kernel(JaggedA
   for (int i = set, buf = 0; i - set < n; i += SETS, buf ^= 1) {
     const int now = r0;
     if (i + SETS < n) {
-      next();
-      if (SETS > 1) next();
+      bool moved = next();
+      if (SETS > 1) moved |= next();
+      if (moved) seek();
       load(buf ^ 1);
     }
     if (k0 < t.len && i < n && !(a.causal && now + BQ - 1 < k0)) {
@@ -244,7 +258,7 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dkv_kernel(JaggedA
 template <typename T, int DP, int BN, int BYTES, int QW, int SETS>
 static void dq_run(JaggedAttnArgs a, hipStream_t st) {
   a.slots = jagged_slots(a.rows, a.B, 32 * QW);
-  hipLaunchKernelGGL((jagged_attn_dq_kernel<T, DP, BN, BYTES, QW, SETS>), dim3((unsigned)(a.slots * a.Hkv * a.group)),
+  hipLaunchKernelGGL((jagged_attn_dq_kernel<T, DP, BN, BYTES, QW, SETS>), dim3((unsigned)jagged_grid(a.slots, a.Hkv, a.group)),
                      dim3(64 * QW * SETS), 0, st, a);
 }
 template <typename T, int DP, int BQ, int WANT, int BYTES, int QW, int SETS>
@@ -252,7 +266,7 @@ static void dkv_run(JaggedAttnArgs a, hipStream_t st) {
   a.slots = jagged_slots(a.rows, a.B, 32 * QW);
   a.heads_per_key = a.group;
   a.group = 1;
-  hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, WANT, BYTES, QW, SETS>), dim3((unsigned)(a.slots * a.Hkv)),
+  hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, WANT, BYTES, QW, SETS>), dim3((unsigned)jagged_grid(a.slots, a.Hkv, 1)),
                      dim3(64 * QW * SETS), 0, st, a);
 }
 template <typename T, int DP, int BYTES>

@@ -23,9 +23,9 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedA
   __shared__ u32x4_t lds[SETS * 4 * TILE];
   static_assert(SETS == 1 || sizeof(lds) >= (QW * DT * 16 + 2 * QW) * 256, "a set's sums fit");
   const JaggedWork wk = jagged_work(a, blockIdx.x);
+  if (wk.slot >= a.slots) return;
   const int head = wk.hk * a.group + wk.g, H = a.Hkv * a.group;
-  // later tiles of a causal sequence have more keys: they go first
-  const JaggedTile t = jagged_tile<BM>(a.offsets, a.B, a.rows, a.slots - 1 - wk.slot);
+  const JaggedTile t = jagged_tile<BM, false>(a.offsets, a.B, a.rows, wk.slot);
   if (t.len == 0) return;
   if (t.tail) {
     ja_zero((T*)a.out + ((t.s0 + t.r0) * H + head) * a.dv, (int64_t)H * a.dv, min(BM, t.len - t.r0), a.dv);
@@ -39,11 +39,14 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedA
   const T* vb = (const T*)a.v + t.s0 * a.ld_v + wk.hk * a.hs_v;
   const int keys = a.causal ? min(t.len, t.r0 + BM) : t.len;
   const int first = set * BN, step = SETS * BN;
-  auto load = [&](int k0, int buf) {
-    ja_stage<T, DP, BN, BYTES, QW>(kb, a.ld_k, k0, t.len, a.d, lk + buf);
-    ja_stage<T, DP, BN, BYTES, QW>(vb, a.ld_v, k0, t.len, a.dv, lv + buf);
+  JaStage<T, DP, BN, BYTES, QW> sk, sv;
+  sk.init(kb, a.ld_k, first, t.len, a.d);
+  sv.init(vb, a.ld_v, first, t.len, a.dv);
+  auto load = [&](int buf) {
+    sk.load(ja_lds(lk + buf), step);
+    sv.load(ja_lds(lv + buf), step);
   };
-  if (first < keys) load(first, 0);
+  if (first < keys) load(0);
   JaRows<T, DP, ja_keep<T, DP>> q;
   q.init((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, a.ld_q, q0, t.len, a.d);
   ja_landed();
@@ -53,7 +56,7 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedA
   float m = -INFINITY, l = 0.f;
   // every set makes the same number of rounds, the last one perhaps without a tile
   for (int k0 = first, buf = 0; k0 - first < keys; k0 += step, buf = TILE - buf) {
-    if (k0 + step < keys) load(k0 + step, TILE - buf);
+    if (k0 + step < keys) load(TILE - buf);
     // a wave whose rows are past the end, or before every key of the tile, has nothing here
     if (q0 < t.len && k0 < keys && !(a.causal && k0 > q0 + 31)) {
       f32x16 s[NB];
@@ -132,7 +135,7 @@ int jagged_attn_check(const char* what, JaggedAttnArgs& a, int H, int bf16) {
              "%s: bad sizes", what);
   GR_REQUIRE(a.scale > 0.f && a.scale < INFINITY, "%s: scale must be positive", what);
   GR_REQUIRE(a.rows == 0 || (a.q && a.k && a.v && a.offsets && a.out), "%s: null pointer", what);
-  GR_REQUIRE(a.rows < (1ll << 31) && (a.rows / 32 + a.B + 1) * (int64_t)H < (1ll << 31), "%s: too many tiles", what);
+  GR_REQUIRE(a.rows < (1ll << 31) && (a.rows / 32 + a.B + 9) * (int64_t)H < (1ll << 31), "%s: too many tiles", what);
   const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.dout;
   const int64_t steps = a.ld_q | a.hs_q | a.ld_k | a.hs_k | a.ld_v | a.hs_v | a.d | a.dv;
   // LDS loads of 4 or 16 bytes: bf16 rows of even widths and strides on 4-byte boundaries
@@ -148,7 +151,7 @@ int jagged_attn_check(const char* what, JaggedAttnArgs& a, int H, int bf16) {
 template <typename T, int DP, int BN, int BYTES, int QW, int SETS>
 static void fwd_run(JaggedAttnArgs a, hipStream_t st) {
   a.slots = jagged_slots(a.rows, a.B, 32 * QW);
-  hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, DP, BN, BYTES, QW, SETS>), dim3((unsigned)(a.slots * a.Hkv * a.group)),
+  hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, DP, BN, BYTES, QW, SETS>), dim3((unsigned)jagged_grid(a.slots, a.Hkv, a.group)),
                      dim3(64 * QW * SETS), 0, st, a);
 }
 template <typename T, int DP, int BYTES>
