@@ -454,8 +454,8 @@ __device__ __forceinline__ void ja_zero(T* base, int64_t ld, int n, int width) {
   for (int i = threadIdx.x; i < n * width; i += blockDim.x) base[(int64_t)(i / width) * ld + i % width] = (T)0.f;
 }
 
-// Two sets of waves that each took every other tile join their sums: the second set's
-// accumulators pass through LDS (4 KB a tile and wave; the tiles' own space).
+// Sets of waves that took the tiles in turn join their sums: the other sets' accumulators pass
+// to the first through LDS (4 KB an accumulator and wave; the tiles' own space).
 template <int QW, int DT>
 __device__ __forceinline__ void ja_give(float* lds, const f32x16 (&v)[DT]) {
   float* at = lds + ((wave_id() % QW) * DT * 16) * 64 + (threadIdx.x & 63);
@@ -490,10 +490,13 @@ __device__ __forceinline__ float half_sum(float v) {
 template <typename T, int DP>
 constexpr bool ja_keep = sizeof(T) == 2 || DP <= 128;
 
-// Whether there are at most two tiles of 128 rows for each CU: two wave sets then share a
-// workgroup's tiles.
-inline bool jagged_few(const JaggedAttnArgs& a, int heads) {
-  return (a.rows / 128 + a.B) * heads <= 2 * device_cus();
+// Whether there are at most `per_cu` tiles of 128 rows for each CU.  The fewer the tiles, the
+// more wave sets share a workgroup's: the longest tile's time is what counts then, and with
+// many tiles the joining is only in the way.  Measured over ragged batches (us):
+//   forward / key pass, 24 x 1,499 rows, 8 heads on 2 of 64: 4 waves 45 / 176, 4 sets of two 51 / 106;
+//   2 x 8,192 rows, 4 heads of 128, forward: one set 146, two sets 109; 128 x 700: 87 and 117.
+inline bool jagged_few(const JaggedAttnArgs& a, int heads, int per_cu) {
+  return (a.rows / 128 + a.B) * heads <= per_cu * device_cus();
 }
 // Checks the sizes and fills in the rest of the arguments.
 int jagged_attn_check(const char* what, JaggedAttnArgs& a, int H, int bf16);

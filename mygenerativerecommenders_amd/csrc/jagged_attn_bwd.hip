@@ -22,7 +22,7 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dq_kernel(JaggedAt
   using Tile = JaTile<T, DP>;
   constexpr int BM = 32 * QW, NB = BN / 32, DT = DP / 32, TILE = Tile::size(BN);
   __shared__ u32x4_t lds[SETS * 4 * TILE];
-  static_assert(SETS == 1 || sizeof(lds) >= QW * DT * 16 * 256, "a set's sums fit");
+  static_assert(sizeof(lds) >= (SETS - 1) * QW * DT * 16 * 256, "the other sets' sums fit");
   const JaggedWork wk = jagged_work(a, blockIdx.x);
   if (wk.slot >= a.slots) return;
   const int head = wk.hk * a.group + wk.g, H = a.Hkv * a.group;
@@ -100,11 +100,13 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dq_kernel(JaggedAt
     ja_landed();
   }
   if constexpr (SETS > 1) {
+    constexpr int SUMS = QW * DT * 16 * 64;
     float* sums = reinterpret_cast<float*>(lds);
-    if (set) ja_give<QW>(sums, acc);
+    if (set) ja_give<QW>(sums + (set - 1) * SUMS, acc);
     __syncthreads();
     if (set) return;
-    ja_take<QW>(sums, acc);
+#pragma unroll
+    for (int j = 0; j < SETS - 1; ++j) ja_take<QW>(sums + j * SUMS, acc);
   }
   T* row = dq + (int64_t)(ok ? qi - t.r0 : 0) * H * a.d;
 #pragma unroll
@@ -122,7 +124,7 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dkv_kernel(JaggedA
   constexpr int BM = 32 * QW, NB = BQ / 32, DT = DP / 32, TILE = Tile::size(BQ);
   __shared__ u32x4_t lds[SETS * 4 * TILE];
   __shared__ __attribute__((aligned(16))) float lsum[SETS * 4 * BQ];
-  static_assert(SETS == 1 || sizeof(lds) >= QW * DT * 16 * 256, "a set's sums fit");
+  static_assert(sizeof(lds) >= (SETS - 1) * QW * DT * 16 * 256, "the other sets' sums fit");
   const JaggedWork wk = jagged_work(a, blockIdx.x);
   if (wk.slot >= a.slots) return;  // group 1: an item per key head
   const int hk = wk.hk, group = a.heads_per_key, H = a.Hkv * group;
@@ -158,7 +160,7 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dkv_kernel(JaggedA
     sq.seek((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, r0, t.len, a.d);
     sg.seek((const T*)a.dout + (t.s0 * H + head) * a.dv, r0, t.len, a.dv);
   };
-  if (set) next();  // a set takes every other tile
+  for (int i = 0; i < set; ++i) next();  // a set takes every SETS-th tile
   sq.init((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, a.ld_q, r0, t.len, a.d);
   sg.init((const T*)a.dout + (t.s0 * H + head) * a.dv, (int64_t)H * a.dv, r0, t.len, a.dv);
   auto load = [&](int buf) {
@@ -191,8 +193,9 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dkv_kernel(JaggedA
   for (int i = set, buf = 0; i - set < n; i += SETS, buf ^= 1) {
     const int now = r0;
     if (i + SETS < n) {
-      bool moved = next();
-      if (SETS > 1) moved |= next();
+      bool moved = false;
+#pragma unroll
+      for (int j = 0; j < SETS; ++j) moved |= next();
       if (moved) seek();
       load(buf ^ 1);
     }
@@ -232,18 +235,19 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dkv_kernel(JaggedA
     ja_landed();
   }
   if constexpr (SETS > 1) {
+    constexpr int SUMS = QW * DT * 16 * 64;
     float* sums = reinterpret_cast<float*>(lds);
-    if (WANT & 1) {
-      if (set) ja_give<QW>(sums, av);
+    auto join = [&](auto& v) {
+      if (set) ja_give<QW>(sums + (set - 1) * SUMS, v);
       __syncthreads();
-      if (!set) ja_take<QW>(sums, av);
-      if (WANT & 2) __syncthreads();
-    }
-    if (WANT & 2) {
-      if (set) ja_give<QW>(sums, ak);
-      __syncthreads();
-      if (!set) ja_take<QW>(sums, ak);
-    }
+      if (!set) {
+#pragma unroll
+        for (int j = 0; j < SETS - 1; ++j) ja_take<QW>(sums + j * SUMS, v);
+      }
+    };
+    if (WANT & 1) join(av);
+    if (WANT == 3) __syncthreads();
+    if (WANT & 2) join(ak);
     if (set) return;
   }
   T* krow = dk + (int64_t)(ok ? ki - t.r0 : 0) * a.Hkv * a.d;
@@ -271,8 +275,18 @@ static void dkv_run(JaggedAttnArgs a, hipStream_t st) {
 }
 template <typename T, int DP, int BYTES>
 static void bwd_shape(const JaggedAttnArgs& a, hipStream_t st) {
+  const int H = a.Hkv * a.group;
   if constexpr (sizeof(T) == 4) {
-    if constexpr (DP <= 128) {
+    if constexpr (DP == 64) {
+      if (jagged_few(a, H, 1))
+        dq_run<T, DP, 32, BYTES, 2, 4>(a, st);
+      else
+        dq_run<T, DP, 32, BYTES, 2, 2>(a, st);
+      if (jagged_few(a, a.Hkv, 1))
+        dkv_run<T, DP, 32, 3, BYTES, 2, 4>(a, st);
+      else
+        dkv_run<T, DP, 32, 3, BYTES, 2, 2>(a, st);
+    } else if constexpr (DP == 128) {
       dq_run<T, DP, 32, BYTES, 2, 2>(a, st);
       dkv_run<T, DP, 32, 3, BYTES, 2, 2>(a, st);
     } else {
@@ -281,16 +295,16 @@ static void bwd_shape(const JaggedAttnArgs& a, hipStream_t st) {
       dkv_run<T, DP, 32, 2, BYTES, 4, 1>(a, st);
     }
   } else if constexpr (DP == 64) {
-    if (jagged_few(a, a.Hkv * a.group))
-      dq_run<T, DP, 64, BYTES, 4, 2>(a, st);
+    if (jagged_few(a, H, 2))
+      dq_run<T, DP, 64, BYTES, 2, 4>(a, st);
     else
       dq_run<T, DP, 64, BYTES, 4, 1>(a, st);
-    if (jagged_few(a, a.Hkv))
-      dkv_run<T, DP, 32, 3, BYTES, 2, 2>(a, st);
+    if (jagged_few(a, a.Hkv, 2))
+      dkv_run<T, DP, 32, 3, BYTES, 2, 4>(a, st);
     else
       dkv_run<T, DP, 64, 3, BYTES, 4, 1>(a, st);
   } else if constexpr (DP == 128) {
-    if (jagged_few(a, a.Hkv * a.group))
+    if (jagged_few(a, H, 2))
       dq_run<T, DP, 32, BYTES, 4, 2>(a, st);
     else
       dq_run<T, DP, 32, BYTES, 4, 1>(a, st);

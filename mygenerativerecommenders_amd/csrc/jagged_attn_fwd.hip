@@ -21,7 +21,7 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedA
   using Tile = JaTile<T, DP>;
   constexpr int BM = 32 * QW, NB = BN / 32, DT = DP / 32, TILE = Tile::size(BN);
   __shared__ u32x4_t lds[SETS * 4 * TILE];
-  static_assert(SETS == 1 || sizeof(lds) >= (QW * DT * 16 + 2 * QW) * 256, "a set's sums fit");
+  static_assert(sizeof(lds) >= (SETS - 1) * (QW * DT * 16 + 2 * QW) * 256, "the other sets' sums fit");
   const JaggedWork wk = jagged_work(a, blockIdx.x);
   if (wk.slot >= a.slots) return;
   const int head = wk.hk * a.group + wk.g, H = a.Hkv * a.group;
@@ -105,19 +105,23 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedA
   }
   l = half_sum(l);
   if constexpr (SETS > 1) {
-    float *sums = reinterpret_cast<float*>(lds), *ml = sums + QW * DT * 16 * 64 + (wave % QW) * 128 + lane;
+    constexpr int SUMS = QW * DT * 16 * 64;
+    float *sums = reinterpret_cast<float*>(lds), *ml = sums + (SETS - 1) * SUMS + (wave % QW) * 128 + lane;
     if (set) {
-      ja_give<QW>(sums, o);
-      ml[0] = m;
-      ml[64] = l;
+      ja_give<QW>(sums + (set - 1) * SUMS, o);
+      ml[(set - 1) * QW * 128] = m;
+      ml[(set - 1) * QW * 128 + 64] = l;
     }
     __syncthreads();
     if (set) return;
-    const float top = fmaxf(m, ml[0]), f = __builtin_amdgcn_exp2f((m - top) * a.scale_l2),
-                g = __builtin_amdgcn_exp2f((ml[0] - top) * a.scale_l2);
-    ja_take<QW>(sums, o, f, g);
-    l = l * f + ml[64] * g;
-    m = top;
+#pragma unroll
+    for (int j = 0; j < SETS - 1; ++j) {
+      const float mj = ml[j * QW * 128], top = fmaxf(m, mj), f = __builtin_amdgcn_exp2f((m - top) * a.scale_l2),
+                  g = __builtin_amdgcn_exp2f((mj - top) * a.scale_l2);
+      ja_take<QW>(sums + j * SUMS, o, f, g);
+      l = l * f + ml[j * QW * 128 + 64] * g;
+      m = top;
+    }
   }
   const bool ok = qi < t.len;
   const int64_t out0 = ((t.s0 + (ok ? qi : 0)) * H + head) * a.dv;
@@ -156,14 +160,21 @@ static void fwd_run(JaggedAttnArgs a, hipStream_t st) {
 }
 template <typename T, int DP, int BYTES>
 static void fwd_shape(const JaggedAttnArgs& a, hipStream_t st) {
+  const int H = a.Hkv * a.group;
   if constexpr (sizeof(T) == 4) {
-    if constexpr (DP <= 128)
+    if constexpr (DP == 64) {
+      if (jagged_few(a, H, 1))
+        fwd_run<T, DP, 32, BYTES, 2, 4>(a, st);
+      else
+        fwd_run<T, DP, 32, BYTES, 2, 2>(a, st);
+    } else if constexpr (DP == 128) {
       fwd_run<T, DP, 32, BYTES, 2, 2>(a, st);
-    else
+    } else {
       fwd_run<T, DP, 32, BYTES, 4, 1>(a, st);
+    }
   } else if constexpr (DP <= 128) {
-    if (jagged_few(a, a.Hkv * a.group))
-      fwd_run<T, DP, 64, BYTES, 4, 2>(a, st);
+    if (jagged_few(a, H, 2))
+      fwd_run<T, DP, 64, BYTES, DP == 64 ? 2 : 4, DP == 64 ? 4 : 2>(a, st);
     else
       fwd_run<T, DP, 64, BYTES, 4, 1>(a, st);
   } else {
