@@ -311,10 +311,22 @@ struct JaFrag<__bf16> {
         x[s] = u32x4_t{pack_bf16(p[8 * s], p[8 * s + 1]), pack_bf16(p[8 * s + 2], p[8 * s + 3]),
                        pack_bf16(p[8 * s + 4], p[8 * s + 5]), pack_bf16(p[8 * s + 6], p[8 * s + 7])};
     }
+    // What the rounding of `p` left off.
+    __device__ __forceinline__ Rows low(const f32x16& p) const {
+      f32x16 e;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[8 * s + 2 * i] = p[8 * s + 2 * i] - __uint_as_float(x[s][i] << 16);
+          e[8 * s + 2 * i + 1] = p[8 * s + 2 * i + 1] - __uint_as_float(x[s][i] & 0xFFFF0000u);
+        }
+      return Rows(e);
+    }
     // Transposed reads: lane 4 q + p of a 16-lane group addresses row q, columns 4 p on of a
     // 4 x 16 block and receives column lane % 16 of its 4 rows.
-    template <int DP>
-    __device__ __forceinline__ f32x16 mma(const u32x4_t* tile, int r0, int t, f32x16 c) const {
+    template <int DP, bool LOW = false>
+    __device__ __forceinline__ f32x16 mma(const u32x4_t* tile, int r0, int t, f32x16 c, const Rows* e = nullptr) const {
       using Tile = JaTile<__bf16, DP>;
       const int lane = threadIdx.x & 63, g = lane >> 4, q = (lane & 15) >> 2, p = lane & 3;
       const int row = 4 * (lane >> 5) + q, cl = 2 * (g & 1) + (p >> 1);
@@ -324,6 +336,7 @@ struct JaFrag<__bf16> {
         const u32x2_t a = tr16(reinterpret_cast<const __bf16*>(lo) + 4 * (p & 1)),
                       b = tr16(reinterpret_cast<const __bf16*>(hi) + 4 * (p & 1));
         c = mfma32(u32x4_t{a.x, a.y, b.x, b.y}, x[s], c);
+        if constexpr (LOW) c = mfma32(u32x4_t{a.x, a.y, b.x, b.y}, e->x[s], c);
       }
       return c;
     }

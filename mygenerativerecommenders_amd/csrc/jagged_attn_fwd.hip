@@ -15,7 +15,10 @@
 
 namespace gr {
 
-template <typename T, int DP, int BN, int BYTES, int QW, int SETS>
+// EXACT (bf16, for the backward pass): the probabilities' rounding errors go through the product
+// with V too.  The backward pass subtracts sum(dO O) from dO V^T; left in O, they were a
+// third of dQ's error beyond that of its own type.
+template <typename T, int DP, int BN, int BYTES, int QW, int SETS, bool EXACT>
 __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedAttnArgs a) {
   using F = JaFrag<T>;
   using Tile = JaTile<T, DP>;
@@ -97,8 +100,14 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedA
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const typename F::Rows p(s[b]);
+        if constexpr (EXACT) {
+          const typename F::Rows e = p.low(s[b]);
 #pragma unroll
-        for (int i = 0; i < DT; ++i) o[i] = p.template mma<DP>(lv + buf, 32 * b, i, o[i]);
+          for (int i = 0; i < DT; ++i) o[i] = p.template mma<DP, true>(lv + buf, 32 * b, i, o[i], &e);
+        } else {
+#pragma unroll
+          for (int i = 0; i < DT; ++i) o[i] = p.template mma<DP>(lv + buf, 32 * b, i, o[i]);
+        }
       }
     }
     ja_landed();
@@ -155,8 +164,14 @@ int jagged_attn_check(const char* what, JaggedAttnArgs& a, int H, int bf16) {
 template <typename T, int DP, int BN, int BYTES, int QW, int SETS>
 static void fwd_run(JaggedAttnArgs a, hipStream_t st) {
   a.slots = jagged_slots(a.rows, a.B, 32 * QW);
-  hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, DP, BN, BYTES, QW, SETS>), dim3((unsigned)jagged_grid(a.slots, a.Hkv, a.group)),
-                     dim3(64 * QW * SETS), 0, st, a);
+  const dim3 grid((unsigned)jagged_grid(a.slots, a.Hkv, a.group)), block(64 * QW * SETS);
+  if constexpr (sizeof(T) == 2) {
+    if (a.out_low) {
+      hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, DP, BN, BYTES, QW, SETS, true>), grid, block, 0, st, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((jagged_attn_fwd_kernel<T, DP, BN, BYTES, QW, SETS, false>), grid, block, 0, st, a);
 }
 template <typename T, int DP, int BYTES>
 static void fwd_shape(const JaggedAttnArgs& a, hipStream_t st) {
