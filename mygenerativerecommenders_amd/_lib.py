@@ -84,6 +84,31 @@ def lib():
     return _lib
 
 
+# What libgr_torch.so calls, in the order of its table.
+_BOUND = ("gr_last_error", "gr_layer_norm_fwd", "gr_layer_norm_bwd_workspace_size", "gr_layer_norm_bwd",
+          "gr_jagged_attn_fwd", "gr_jagged_attn_bwd_workspace_size", "gr_jagged_attn_bwd",
+          "gr_adamw8_step")
+NODES_PATH = os.path.join(PKG_DIR, "libgr_torch.so")
+_nodes = None
+
+
+def nodes():
+    """The torch operators of ``libgr_torch.so`` (csrc/torch/nodes.cpp), bound to ``lib()``."""
+    global _nodes
+    if _nodes is not None:
+        return _nodes
+    L = lib()
+    with _lock:
+        if _nodes is None:
+            if not os.path.exists(NODES_PATH):
+                raise RuntimeError(f"{NODES_PATH} is missing: build it with `python -c 'import "
+                                   "__graft_entry__ as g; g.build()'`.")
+            torch.ops.load_library(NODES_PATH)
+            torch.ops.gr_amd.bind([ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in _BOUND])
+            _nodes = torch.ops.gr_amd
+    return _nodes
+
+
 class GrError(RuntimeError):
     pass
 

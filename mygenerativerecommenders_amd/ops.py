@@ -18,7 +18,6 @@ Reference map (``src/generative_recommenders_pl/models/``):
 from __future__ import annotations
 
 
-import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -196,74 +195,6 @@ def l2_normalize(x: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
 _FLOATS = (torch.float32, torch.bfloat16)
 
 
-def _on(device):
-    """The device's own context where it is not the current one: launches and the current
-    stream then are that device's."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
-def _rows_of(x, D: int):
-    """x as (rows, D) with contiguous columns: a view wherever its strides allow."""
-    if x.dim() == 2 and x.stride(1) == 1:
-        return x
-    x2 = x.reshape(-1, D)
-    return x2 if D == 1 or x2.stride(1) == 1 else x2.contiguous()
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps: float, grad_on: bool):
-        D = x.shape[-1]
-        x2 = _rows_of(x, D)
-        rows = x2.shape[0]
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device) if grad_on else None
-        affine = weight if weight is not None else bias
-        types = int(x.dtype == torch.bfloat16) + 2 * int(affine is not None and affine.dtype == torch.bfloat16)
-        with _on(x.device):
-            _lib.call("gr_layer_norm_fwd", x2.data_ptr(), x2.stride(0), rows, D, _lib.ptr(weight),
-                      _lib.ptr(bias), types, eps, y.data_ptr(), D, _lib.ptr(stats), _stream())
-        if grad_on:
-            ctx.save_for_backward(x, weight, bias, stats)
-        ctx.types, ctx.eps = types, eps
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
-        D = x.shape[-1]
-        want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        if torch.is_grad_enabled():  # create_graph: differentiable torch operations
-            return (*_layer_norm_grads(x, weight, bias, ctx.eps, dy, want_x, want_w, want_b), None, None)
-        x2, g = _rows_of(x, D), _rows_of(dy, D)
-        rows = x2.shape[0]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
-        dw = torch.empty_like(weight) if want_w else None
-        db = torch.empty_like(bias) if want_b else None
-        n = _lib.lib().gr_layer_norm_bwd_workspace_size(rows, D, ctx.types) if want_w or want_b else 0
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-        with _on(x.device):
-            _lib.call("gr_layer_norm_bwd", g.data_ptr(), g.stride(0), x2.data_ptr(), x2.stride(0), rows,
-                      D, _lib.ptr(weight), ctx.types, stats.data_ptr(), _lib.ptr(dx), D, _lib.ptr(dw),
-                      _lib.ptr(db), _lib.ptr(ws), n, _stream())
-        return dx, dw, db, None, None
-
-
-def _layer_norm_grads(x, weight, bias, eps, dy, want_x, want_w, want_b):
-    xf, g = x.float(), dy.float()
-    c = xf - xf.mean(-1, keepdim=True)
-    r = torch.rsqrt((c * c).mean(-1, keepdim=True) + eps)
-    xh = c * r
-    gw = g if weight is None else g * weight.float()
-    dx = r * (gw - gw.mean(-1, keepdim=True) - xh * (gw * xh).mean(-1, keepdim=True))
-    D = x.shape[-1]
-    return (dx.to(x.dtype) if want_x else None,
-            (g * xh).reshape(-1, D).sum(0).to(weight.dtype) if want_w else None,
-            g.reshape(-1, D).sum(0).to(bias.dtype) if want_b else None)
-
-
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                bias: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension, forward and
@@ -283,9 +214,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
             raise TypeError("layer_norm: weight and bias must be float32 or bfloat16, both the same")
         if tuple(t.shape) != (x.shape[-1],) or t.device != x.device:
             raise ValueError(f"layer_norm: weight and bias must be ({x.shape[-1]},) tensors on {x.device}")
-    grad_on = torch.is_grad_enabled() and any(t.requires_grad for t in (x, *params))
-    return _LayerNorm.apply(x, None if weight is None else weight.contiguous(),
-                            None if bias is None else bias.contiguous(), float(eps), grad_on)
+    return _lib.nodes().layer_norm.default(x, None if weight is None else weight.contiguous(),
+                                           None if bias is None else bias.contiguous(), float(eps))
 
 
 # ------------------------------------------------------------------ relative-time buckets
@@ -1288,55 +1218,6 @@ def stu_softmax_layer(x, offsets, bias, w_uvqk, w_o, b_o, geo: STUGeometry, seed
 
 # ------------------------------------------------------------------ per-head softmax attention
 
-def _columns(x):
-    """x itself where the kernels read it in place: contiguous columns, row strides below 2^22,
-    for bfloat16 even strides and a start on a 4-byte boundary; else a contiguous copy."""
-    s = x.stride()
-    ok = s[2] == 1 and 0 <= s[0] < 1 << 22
-    if x.dtype == torch.bfloat16:
-        ok = ok and s[0] % 2 == 0 and s[1] % 2 == 0 and x.data_ptr() % 4 == 0
-    return x if ok else x.contiguous()
-
-
-class _JaggedAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, offsets, causal: bool, scale: float, grad_on: bool):
-        q, k, v = _columns(q), _columns(k), _columns(v)
-        rows, H, d = q.shape
-        Hkv, dv = k.shape[1], v.shape[2]
-        out = torch.empty(rows, H, dv, dtype=q.dtype, device=q.device)
-        lse = torch.empty(H, rows, dtype=torch.float32, device=q.device) if grad_on else None
-        low = torch.empty_like(out) if grad_on and q.dtype == torch.bfloat16 else None
-        ctx.call = (offsets.numel() - 1, rows, H, Hkv, d, dv, int(causal), scale,
-                    int(q.dtype == torch.bfloat16))
-        with _on(q.device):
-            _lib.call("gr_jagged_attn_fwd", *_strided(q), *_strided(k), *_strided(v),
-                      offsets.data_ptr(), *ctx.call, out.data_ptr(), _lib.ptr(low),
-                      _lib.ptr(lse), _stream())
-        if grad_on:
-            ctx.save_for_backward(q, k, v, offsets, out, low, lse)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
-        q, k, v, offsets, out, low, lse = ctx.saved_tensors
-        dout = dout.contiguous()
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        n = _lib.lib().gr_jagged_attn_bwd_workspace_size(q.shape[0], q.shape[1])
-        ws = torch.empty(max(n, 4), dtype=torch.uint8, device=q.device)
-        with _on(q.device):
-            _lib.call("gr_jagged_attn_bwd", *_strided(q), *_strided(k), *_strided(v),
-                      offsets.data_ptr(), *ctx.call, out.data_ptr(), _lib.ptr(low), lse.data_ptr(),
-                      dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(),
-                      n, _stream())
-        return dq, dk, dv, None, None, None, None
-
-
-def _strided(x):
-    return x.data_ptr(), x.stride(0), x.stride(1)
-
-
 def jagged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
                      causal: bool = True, scale: Optional[float] = None) -> torch.Tensor:
     """Softmax attention of each head over the rows of its own sequence, forward and backward
@@ -1374,8 +1255,7 @@ def jagged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     # heads narrower than 16 bytes, and bf16 heads of odd widths, get zero columns
     dv = v.shape[2]
     q, k, v = _even(q, d), _even(k, d), _even(v, dv)
-    grad_on = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v))
-    out = _JaggedAttention.apply(q, k, v, offsets.to(torch.int64).contiguous(), bool(causal), scale, grad_on)
+    out = _lib.nodes().jagged_attention.default(q, k, v, offsets.to(torch.int64).contiguous(), bool(causal), scale)
     return out if out.shape[2] == dv else out[..., :dv]
 
 

@@ -21,7 +21,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-from . import _lib, ops
+from . import _lib
 
 
 _BLOCK = 64  # elements that share a scale of an 8-bit moment
@@ -91,7 +91,6 @@ class FlatAdamW(torch.optim.Optimizer):
                              "exp_avg_sq": fs["exp_avg_sq"][off:off + n].view_as(p),
                              "exp_avg_sq_scale": fs["exp_avg_sq_scale"][blocks]}
         fs["done"] = torch.zeros(1040, dtype=torch.int32, device=dev)  # 65 counters, 64 bytes apart
-        fs["offs"] = offs
         self._flat[gi] = fs
         return fs
 
@@ -102,7 +101,7 @@ class FlatAdamW(torch.optim.Optimizer):
         64 (8 bits), in the order of the group's parameters."""
         fs = self._group_state(group, self.param_groups[group])
         if self._bits == 8:
-            return {n: t for n, t in fs.items() if n not in ("done", "offs")}
+            return {n: t for n, t in fs.items() if n != "done"}
         return {"exp_avg": fs["m"], "exp_avg_sq": fs["v"], "step": fs["step"]}
 
     def load_state_dict(self, state_dict: dict) -> None:
@@ -141,6 +140,13 @@ class FlatAdamW(torch.optim.Optimizer):
                 loss = closure()
         for gi, group in enumerate(self.param_groups):
             params = group["params"]
+            if self._bits == 8 and params:
+                fs = self._flat.get(gi) or self._group_state(gi, group)
+                _lib.nodes().adamw8_step.default(
+                    params, fs["exp_avg"], fs["exp_avg_scale"], fs["exp_avg_sq"], fs["exp_avg_sq_scale"],
+                    fs["step"], fs["done"], float(group["lr"]), float(group["betas"][0]),
+                    float(group["betas"][1]), float(group["eps"]), float(group["weight_decay"]))
+                continue
             if not params or all(p.grad is None for p in params):
                 continue
             fs = self._group_state(gi, group)
@@ -157,16 +163,9 @@ class FlatAdamW(torch.optim.Optimizer):
                     raise TypeError("FlatAdamW: dense contiguous fp32 gradients expected")
                 pp[i], gp[i], ne[i] = p.data_ptr(), g.data_ptr(), p.numel()
             b1, b2 = group["betas"]
-            hyper = (float(group["lr"]), float(b1), float(b2), float(group["eps"]),
-                     float(group["weight_decay"]))
-            lists = (pp.ctypes.data, gp.ctypes.data, fs["offs"].ctypes.data, ne.ctypes.data, n)
-            if self._bits == 8:
-                with ops._on(params[0].device):
-                    _lib.call("gr_adamw8_step", *lists, fs["exp_avg"].data_ptr(),
-                              fs["exp_avg_scale"].data_ptr(), fs["exp_avg_sq"].data_ptr(),
-                              fs["exp_avg_sq_scale"].data_ptr(), fs["step"].data_ptr(),
-                              fs["done"].data_ptr(), *hyper, _lib.stream_handle())
-                continue
-            _lib.call("gr_adamw_step", *lists, fs["m"].data_ptr(), fs["v"].data_ptr(),
-                      fs["step"].data_ptr(), fs["done"].data_ptr(), *hyper, _lib.stream_handle())
+            _lib.call("gr_adamw_step", pp.ctypes.data, gp.ctypes.data, fs["offs"].ctypes.data,
+                      ne.ctypes.data, n, fs["m"].data_ptr(), fs["v"].data_ptr(),
+                      fs["step"].data_ptr(), fs["done"].data_ptr(), float(group["lr"]), float(b1),
+                      float(b2), float(group["eps"]), float(group["weight_decay"]),
+                      _lib.stream_handle())
         return loss
