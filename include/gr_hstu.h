@@ -320,9 +320,11 @@ GR_API int gr_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64
  * q (rows, H, d), k (rows, Hkv, d), v (rows, Hkv, dv): bf16 (bf16 != 0) or fp32, element
  * strides ld_* of a row (in [0, 2^22)) and hs_* of a head, columns contiguous, no alignment
  * beyond the element's for fp32, even strides and widths from 4-byte boundaries on for bf16;
- * 16 bytes <= d, dv <= 256 elements, H a multiple of Hkv, scale > 0.  out, dout (rows, H, dv), dq
- * (rows, H, d), dk (rows, Hkv, d), dvv (rows, Hkv, dv) are contiguous.  Rows past
- * offsets[B] get zeros; offsets are clamped to [0, rows].  lse (H, rows): log2 of each row's
+ * 16 bytes <= d, dv <= 256 elements, H a multiple of Hkv, H dv < 2^22, scale > 0.  out, dout (rows, H, dv), dq
+ * (rows, H, d), dk (rows, Hkv, d), dvv (rows, Hkv, dv) are contiguous.  offsets ascend; rows
+ * before offsets[0] and from offsets[B] on get zeros and are not read; offsets are clamped to
+ * [0, rows].  An infinity or NaN in a row can reach every row of its sequence and key head, those
+ * before it included, and no other.  lse (H, rows): log2 of each row's
  * sum of exp(scaled scores); out_low (bf16 only, as out): what rounding left off out, so that
  * the backward's sum(dout out) is that of the unrounded rows.  The backward needs both
  * (forward: NULL if there is none).

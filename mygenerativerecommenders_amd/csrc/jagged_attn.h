@@ -71,29 +71,30 @@ __device__ __forceinline__ int wave_isum(int v) {
          __builtin_amdgcn_readlane(v, 48);
 }
 
-// Tile `slot` of the jagged rows in tiles of BM rows that never cross a sequence; the rows past
-// the last sequence are tiled as one more (`tail`).  The host knows neither lengths nor tile
-// counts, only that rows / BM + B + 1 slots are enough.  Offsets are clamped to the rows.
+// Tile `slot` of the jagged rows in tiles of BM rows that never cross a sequence; the rows before
+// the first and past the last sequence are tiled as one more each (`none`).  The host knows neither
+// lengths nor tile counts, only that rows / BM + B + 2 slots are enough.  Offsets are clamped to
+// the rows.
 //
 // Up to 255 sequences the wave holds them all, and slots run from the heavy tiles to the light
 // ones: level n of a sequence is the tile that meets n tiles of a causal sequence's other side
 // (`keys`: the key rows' pass, where that is the n-th from the end), slots go down the levels
 // and through the sequences that reach them.  Workgroups start in that order, so the longest
 // do not run alone at the end.  With more sequences, sequence b owns the slots from
-// offsets[b] / BM + b on, found by a search over the offsets, 64 at a time.
+// offsets[b] / BM + b + 1 on, found by a search over the offsets, 64 at a time.
 struct JaggedTile {
   int64_t s0;  // first row of the sequence
   int len;     // its length (0: the slot holds no tile)
   int r0;      // first row of the tile in the sequence
-  bool tail;   // rows of no sequence
+  bool none;   // rows of no sequence
 };
-inline int64_t jagged_slots(int64_t rows, int B, int bm) { return rows / bm + B + 1; }
+inline int64_t jagged_slots(int64_t rows, int B, int bm) { return rows / bm + B + 2; }
 __device__ __forceinline__ int64_t ja_clamp(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
 template <int BM, bool KEYS>
 __device__ __forceinline__ JaggedTile jagged_tile(const int64_t* offsets, int B, int64_t rows, int64_t slot) {
   const int lane = threadIdx.x & 63;
   JaggedTile t;
-  t.tail = false;
+  t.none = false;
   if (B < 256) {
     int first[4], tiles[4], lens[4], total = 0;  // rows < 2^31
 #pragma unroll
@@ -115,10 +116,13 @@ __device__ __forceinline__ JaggedTile jagged_tile(const int64_t* offsets, int B,
     };
     total = above(1);
     if (slot >= total) {
-      const int64_t end = ja_clamp(B > 0 ? offsets[B] : 0, 0, rows), r0 = (slot - total) * BM;
-      t.tail = true;
-      t.s0 = end;
-      t.len = r0 < rows - end ? (int)(rows - end) : 0;
+      const int64_t start = ja_clamp(B > 0 ? offsets[0] : 0, 0, rows), end = ja_clamp(B > 0 ? offsets[B] : 0, start, rows);
+      const int64_t before = (start + BM - 1) / BM, i = slot - total;
+      const bool head = i < before;
+      const int64_t r0 = (head ? i : i - before) * BM, n = head ? start : rows - end;
+      t.none = true;
+      t.s0 = head ? 0 : end;
+      t.len = r0 < n ? (int)n : 0;
       t.r0 = (int)r0;
       return t;
     }
@@ -150,18 +154,19 @@ __device__ __forceinline__ JaggedTile jagged_tile(const int64_t* offsets, int B,
     }
     return t;
   }
-  int lo = 0, hi = B + 1;
+  auto start = [&](int i) { return i > 0 ? ja_clamp(offsets[i - 1], 0, rows) : 0; };  // of sequence i - 1
+  int lo = 0, hi = B + 2;
   while (hi - lo > 1) {
     const int step = (hi - lo + 63) >> 6;
     const int i = lo + lane * step;
-    const bool le = i < hi && ja_clamp(offsets[i < hi ? i : B], 0, rows) / BM + i <= slot;
+    const bool le = i < hi && start(i < hi ? i : 0) / BM + i <= slot;
     const int c = __popcll(__ballot(le));
     lo += (c > 0 ? c - 1 : 0) * step;
     hi = hi < lo + step ? hi : lo + step;
   }
-  t.s0 = ja_clamp(offsets[lo], 0, rows);
-  t.tail = lo == B;
-  const int64_t end = t.tail ? rows : ja_clamp(offsets[lo + 1], t.s0, rows);
+  t.s0 = start(lo);
+  t.none = lo == 0 || lo == B + 1;
+  const int64_t end = lo == B + 1 ? rows : ja_clamp(offsets[lo], t.s0, rows);
   const int64_t r0 = (slot - lo - t.s0 / BM) * BM;
   t.len = r0 >= 0 && r0 < end - t.s0 ? (int)(end - t.s0) : 0;
   t.r0 = (int)r0;

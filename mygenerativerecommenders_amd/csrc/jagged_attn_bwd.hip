@@ -29,7 +29,7 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dq_kernel(JaggedAt
   const JaggedTile t = jagged_tile<BM, false>(a.offsets, a.B, a.rows, wk.slot);
   if (t.len == 0) return;
   T* dq = (T*)a.dq + ((t.s0 + t.r0) * H + head) * a.d;
-  if (t.tail) {
+  if (t.none) {
     ja_zero(dq, (int64_t)H * a.d, min(BM, t.len - t.r0), a.d);
     return;
   }
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dkv_kernel(JaggedA
   if (t.len == 0) return;
   T* dk = (T*)a.dk + ((t.s0 + t.r0) * a.Hkv + hk) * a.d;
   T* dv = (T*)a.dvv + ((t.s0 + t.r0) * a.Hkv + hk) * a.dv;
-  if (t.tail) {
+  if (t.none) {
     if (WANT & 2) ja_zero(dk, (int64_t)a.Hkv * a.d, min(BM, t.len - t.r0), a.d);
     if (WANT & 1) ja_zero(dv, (int64_t)a.Hkv * a.dv, min(BM, t.len - t.r0), a.dv);
     return;

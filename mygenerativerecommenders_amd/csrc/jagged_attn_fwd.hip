@@ -30,7 +30,7 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedA
   const int head = wk.hk * a.group + wk.g, H = a.Hkv * a.group;
   const JaggedTile t = jagged_tile<BM, false>(a.offsets, a.B, a.rows, wk.slot);
   if (t.len == 0) return;
-  if (t.tail) {
+  if (t.none) {
     ja_zero((T*)a.out + ((t.s0 + t.r0) * H + head) * a.dv, (int64_t)H * a.dv, min(BM, t.len - t.r0), a.dv);
     return;
   }
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedA
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[i] *= f;
       }
-      const float mc = m * a.scale_l2;
+      const float mc = m == -INFINITY ? 0.f : m * a.scale_l2;  // nothing but -inf so far: no terms
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -125,8 +125,9 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedA
     if (set) return;
 #pragma unroll
     for (int j = 0; j < SETS - 1; ++j) {
-      const float mj = ml[j * QW * 128], top = fmaxf(m, mj), f = __builtin_amdgcn_exp2f((m - top) * a.scale_l2),
-                  g = __builtin_amdgcn_exp2f((mj - top) * a.scale_l2);
+      const float mj = ml[j * QW * 128], top = fmaxf(m, mj);
+      const float f = m == top ? 1.f : __builtin_amdgcn_exp2f((m - top) * a.scale_l2);  // both may be -inf
+      const float g = mj == top ? 1.f : __builtin_amdgcn_exp2f((mj - top) * a.scale_l2);
       ja_take<QW>(sums + j * SUMS, o, f, g);
       l = l * f + ml[j * QW * 128 + 64] * g;
       m = top;
@@ -148,7 +149,7 @@ int jagged_attn_check(const char* what, JaggedAttnArgs& a, int H, int bf16) {
              "%s: bad sizes", what);
   GR_REQUIRE(a.scale > 0.f && a.scale < INFINITY, "%s: scale must be positive", what);
   GR_REQUIRE(a.rows == 0 || (a.q && a.k && a.v && a.offsets && a.out), "%s: null pointer", what);
-  GR_REQUIRE(a.rows < (1ll << 31) && (a.rows / 32 + a.B + 9) * (int64_t)H < (1ll << 31), "%s: too many tiles", what);
+  GR_REQUIRE(a.rows < (1ll << 31) && (a.rows / 32 + a.B + 10) * (int64_t)H < (1ll << 31), "%s: too many tiles", what);
   const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.dout;
   const int64_t steps = a.ld_q | a.hs_q | a.ld_k | a.hs_k | a.ld_v | a.hs_v | a.d | a.dv;
   // LDS loads of 4 or 16 bytes: bf16 rows of even widths and strides on 4-byte boundaries
@@ -156,6 +157,7 @@ int jagged_attn_check(const char* what, JaggedAttnArgs& a, int H, int bf16) {
   GR_REQUIRE(at % 4 == 0 && (!bf16 || steps % 2 == 0), "%s: bf16 rows must be pairs on 4-byte boundaries", what);
   GR_REQUIRE(a.rows == 0 || (a.ld_q >= 0 && a.ld_q < far && a.ld_k >= 0 && a.ld_k < far && a.ld_v >= 0 && a.ld_v < far),
              "%s: row strides outside [0, 2^22)", what);
+  GR_REQUIRE((int64_t)H * a.dv < far, "%s: output rows of 2^22 elements and more", what);
   a.wide = at % 16 == 0 && steps % least == 0;
   a.group = H / a.Hkv;
     return 0;

@@ -1229,8 +1229,9 @@ def jagged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     gives them; they are not read on the host).  float32 or bfloat16, 1 <= d, dv <= 256, H a
     multiple of Hkv (query head h reads key head h' = h // (H // Hkv)); rows and heads of any
     stride, so column slices of one projection are read in place.  ``scale`` > 0, 1 / sqrt(d)
-    by default.  Returns (rows, H, dv) of q's type; rows past offsets[B] are zero, and so are
-    their gradients.  Softmax and sums are fp32; bfloat16 probabilities enter the products
+    by default.  Returns (rows, H, dv) of q's type; rows before offsets[0] and from offsets[B] on are
+    zero, and so are their gradients.  H dv < 2^22.  An infinity or NaN in a row can reach every
+    row of its sequence and key head, those before it included, and no other.  Softmax and sums are fp32; bfloat16 probabilities enter the products
     rounded to bfloat16.  No atomics: the same bits every run."""
     _lib.require_gpu(q, k, v, offsets)
     if q.dtype not in _FLOATS or k.dtype != q.dtype or v.dtype != q.dtype:

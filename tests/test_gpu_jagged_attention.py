@@ -136,6 +136,51 @@ def test_rows_of_no_sequence_are_zero_and_never_read(d, dtype):
 
 
 @DTYPES
+@pytest.mark.parametrize("many", [0, 400])
+def test_some_sequences_of_a_batch(many, dtype):
+    """A slice of the offsets: the rows before its first sequence are of no sequence either."""
+    lengths = [140, 33] + [50, 0, 129] + [1] * many + [70]
+    q, k, v, offsets, dout = make(lengths, 2, 1, 40, 40, dtype)
+    ends = offsets[2:6 + many]
+    lo, hi = int(ends[0]), int(ends[-1])
+    assert lo == 173 and hi == lo + 179 + many
+    want = run(q[lo:hi], k[lo:hi], v[lo:hi], ends - lo, dout[lo:hi])
+    q, k, v, dout = (t.clone() for t in (q, k, v, dout))
+    for t in (q, k, v, dout):
+        t[:lo] = t[hi:] = float("nan")
+    for x, y in zip(run(q, k, v, ends, dout), want):
+        assert torch.equal(x[lo:hi], y) and (x[:lo] == 0).all() and (x[hi:] == 0).all()
+
+
+@DTYPES
+@pytest.mark.parametrize("d", [40, 128, 256])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+def test_scores_of_minus_infinity(causal, d, dtype):
+    """Keys whose score is -inf, more of them than any tile holds: no part of the sums.  Rows that
+    see no other key are NaN, as a softmax over nothing is."""
+    q, k, v, offsets, dout = make([300, 500], 1, 1, d, d, dtype)
+    q, k = q.abs() + 1, k.clone()
+    k[:280, 0, 0] = -math.inf
+    out = run(q, k, v, offsets, dout, causal=causal)[0]
+    q0, k0 = q.clone(), k.clone()
+    k0[:280, 0, 0] = 0
+    S = d ** -0.5 * (q0[:300, 0].double() @ k0[:300, 0].double().T)
+    S[:, :280] = -math.inf
+    if causal:
+        S = S.masked_fill(~torch.ones(300, 300, dtype=torch.bool, device="cuda").tril(), -math.inf)
+    want = torch.softmax(S, -1) @ v[:300, 0].double()
+    first = 280 if causal else 0
+    assert torch.isnan(out[:first]).all() and torch.isfinite(out[first:]).all()
+    b = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+    err = ((d + 2) * U * d ** -0.5 * (q0[:300, 0].double() @ k0[:300, 0].double().abs().T)).amax()
+    r = 2 * err + (8 + 300 + 2 * S[S.isfinite()].abs().amax()) * U
+    P, V = torch.softmax(S, -1), v[:300, 0].double()
+    lim = (r + b + 300 * U) * (P @ V.abs()) + (b + 4 * U) * want.abs()
+    assert ((out[first:300, 0].double() - want[first:]).abs() <= lim[first:]).all()
+    assert torch.equal(out[300:], run(q[300:], k[300:], v[300:], offsets[1:] - 300, dout[300:], causal=causal)[0])
+
+
+@DTYPES
 def test_neighbours_do_not_leak(dtype):
     """Infinities and NaN stay in their sequence and key head."""
     q, k, v, offsets, dout = make([70, 100, 45], 4, 2, 50, 50, dtype)

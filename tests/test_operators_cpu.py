@@ -22,7 +22,7 @@ def attn(**kw):
                                  dict(H=0), dict(Hkv=0), dict(H=3, Hkv=2), dict(d=3), dict(d=7, bf16=1), dict(d=257), dict(dv=0), dict(dv=300),
                                  dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
                                  dict(q=P + 2), dict(ld_k=-8), dict(ld_v=1 << 22), dict(ld_q=9, bf16=1), dict(hs_k=9, bf16=1),
-                                 dict(d=9, bf16=1),
+                                 dict(d=9, bf16=1), dict(H=1 << 15, Hkv=1 << 15, dv=128),
                                  dict(rows=1 << 31), dict(rows=1 << 30, H=4096, Hkv=4096)], ids=str)
 def test_attention_refuses(bad):
     with pytest.raises(_lib.GrError, match="gr_jagged_attn_fwd"):
