@@ -513,8 +513,13 @@ constexpr bool ja_keep = sizeof(T) == 2 || DP <= 128;
 // many tiles the joining is only in the way.  Measured over ragged batches (us):
 //   forward / key pass, 24 x 1,499 rows, 8 heads on 2 of 64: 4 waves 45 / 176, 4 sets of two 51 / 106;
 //   2 x 8,192 rows, 4 heads of 128, forward: one set 146, two sets 109; 128 x 700: 87 and 117.
-inline bool jagged_few(const JaggedAttnArgs& a, int heads, int per_cu) {
-  return (a.rows / 128 + a.B) * heads <= per_cu * device_cus();
+// At width 256 a workgroup of two sets fills a CU's LDS and one of a single set half of it, and then
+// a SIMD has two waves (forward / dQ / key passes, us):
+//   32 x 2,028, 1 head (298 tiles): two sets 86 / 104 / 203, one set of four waves 117 / 135 / 313;
+//   24 x 1,000, 2 heads (422): 88 / 107 / 197 and 71 / 88 / 174; 128 x 996, 4 heads: 444 / 542 / 917
+//   and 263 / 455 / 640.
+inline bool jagged_few(const JaggedAttnArgs& a, int heads, float per_cu) {
+  return (float)((a.rows / 128 + a.B) * heads) <= per_cu * device_cus();
 }
 // Checks the sizes and fills in the rest of the arguments.
 int jagged_attn_check(const char* what, JaggedAttnArgs& a, int H, int bf16);

@@ -310,9 +310,17 @@ static void bwd_shape(const JaggedAttnArgs& a, hipStream_t st) {
       dq_run<T, DP, 32, BYTES, 4, 1>(a, st);
     dkv_run<T, DP, 32, 3, BYTES, 2, 2>(a, st);
   } else {
-    dq_run<T, DP, 32, BYTES, 2, 2>(a, st);
-    dkv_run<T, DP, 32, 1, BYTES, 2, 2>(a, st);
-    dkv_run<T, DP, 32, 2, BYTES, 2, 2>(a, st);
+    if (jagged_few(a, H, 1.5f))
+      dq_run<T, DP, 32, BYTES, 2, 2>(a, st);
+    else
+      dq_run<T, DP, 32, BYTES, 4, 1>(a, st);
+    if (jagged_few(a, a.Hkv, 1.5f)) {
+      dkv_run<T, DP, 32, 1, BYTES, 2, 2>(a, st);
+      dkv_run<T, DP, 32, 2, BYTES, 2, 2>(a, st);
+    } else {
+      dkv_run<T, DP, 32, 1, BYTES, 4, 1>(a, st);
+      dkv_run<T, DP, 32, 2, BYTES, 4, 1>(a, st);
+    }
   }
 }
 template <typename T, int BYTES>

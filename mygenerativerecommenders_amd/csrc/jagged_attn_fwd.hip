@@ -194,8 +194,10 @@ static void fwd_shape(const JaggedAttnArgs& a, hipStream_t st) {
       fwd_run<T, DP, 64, BYTES, DP == 64 ? 2 : 4, DP == 64 ? 4 : 2>(a, st);
     else
       fwd_run<T, DP, 64, BYTES, 4, 1>(a, st);
-  } else {
+  } else if (jagged_few(a, H, 1.5f)) {
     fwd_run<T, DP, 32, BYTES, 2, 2>(a, st);
+  } else {
+    fwd_run<T, DP, 32, BYTES, 4, 1>(a, st);
   }
 }
 template <typename T, int BYTES>

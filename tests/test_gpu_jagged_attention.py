@@ -123,6 +123,12 @@ def test_many_short_sequences(dtype):
 
 
 @DTYPES
+@pytest.mark.parametrize("d", [62, 128, 256])
+def test_more_tiles_than_the_chip_holds(d, dtype):
+    check(*make([300] + [(37 * i) % 150 for i in range(240)], 4, 2, d, d, dtype))
+
+
+@DTYPES
 @pytest.mark.parametrize("d", [50, 256])
 def test_rows_of_no_sequence_are_zero_and_never_read(d, dtype):
     q, k, v, offsets, dout = make([40, 0, 129], 2, 1, d, d, dtype, spare=300)
