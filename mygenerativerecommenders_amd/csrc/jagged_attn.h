@@ -292,8 +292,21 @@ struct JaStage {
     left -= (int64_t)rows * row;
   }
 };
-__device__ __forceinline__ uint32_t ja_lds(const u32x4_t* tile) {
-  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const u32x4_t*)tile;
+template <typename V>
+__device__ __forceinline__ uint32_t ja_lds(const V* at) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const V*)at;
+}
+// The same for one float a lane (lanes < N of a wave): p[0 .. left - 1], zeros past them.
+template <int N>
+__device__ __forceinline__ void ja_stage_floats(const float* p, int left, uint32_t lds) {
+  const uint64_t at = (uint64_t)p;
+  const u32x4_t desc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xFFFFu, (uint32_t)min(left, N) * 4u, 0x00020000u};
+  const uint32_t base = __builtin_amdgcn_readfirstlane(lds);
+  const int lane = threadIdx.x & 63;
+  uint32_t keep;
+  if (N == 64 || lane < N)
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "s"(base), "v"(4 * lane), "s"(desc) : "memory");
 }
 __device__ __forceinline__ void ja_landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -513,6 +526,8 @@ constexpr bool ja_keep = sizeof(T) == 2 || DP <= 128;
 // many tiles the joining is only in the way.  Measured over ragged batches (us):
 //   forward / key pass, 24 x 1,499 rows, 8 heads on 2 of 64: 4 waves 45 / 176, 4 sets of two 51 / 106;
 //   2 x 8,192 rows, 4 heads of 128, forward: one set 146, two sets 109; 128 x 700: 87 and 117.
+// Key pass at width 128: 24 x 1,000 rows, 4 heads (488 tiles): two sets 44, one 62; 128 x 996, 8 heads on
+// one (653): 275 and 406; 200 x 100, 2 heads (712): 28 and 21; 128 x 996, 4 heads (2,612): 239 and 192.
 // At width 256 a workgroup of two sets fills a CU's LDS and one of a single set half of it, and then
 // a SIMD has two waves (forward / dQ / key passes, us):
 //   32 x 2,028, 1 head (298 tiles): two sets 86 / 104 / 203, one set of four waves 117 / 135 / 313;

@@ -116,9 +116,11 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dq_kernel(JaggedAt
 // dK, dV: one workgroup per 128 key rows and key head, a wave per 32 keys, tiles of BQ query
 // rows of each query head of the group in turn.  WANT: 1 = dV, 2 = dK, 3 = both in one launch;
 // heads wider than 128 take a launch for each, as both results' accumulators and the
-// keys' fragments do not fit the registers together.
+// keys' fragments do not fit the registers together.  bf16 at width 128 fits two waves a SIMD
+// where the compiler is held to it (not with two sets and loads of 4 bytes, whose lanes have more
+// addresses): 128 sequences of up to 996 rows, 4 heads, 334 us -> 192.
 template <typename T, int DP, int BQ, int WANT, int BYTES, int QW, int SETS>
-__global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dkv_kernel(JaggedAttnArgs a) {
+__global__ __launch_bounds__(64 * QW * SETS, sizeof(T) == 2 && DP == 128 && (BYTES == 16 || SETS == 1) ? 2 : 1) void jagged_attn_dkv_kernel(JaggedAttnArgs a) {
   using F = JaFrag<T>;
   using Tile = JaTile<T, DP>;
   constexpr int BM = 32 * QW, NB = BQ / 32, DT = DP / 32, TILE = Tile::size(BQ);
@@ -138,13 +140,12 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dkv_kernel(JaggedA
     return;
   }
   const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5;
-  const int set = SETS > 1 ? wave / QW : 0, tid = threadIdx.x % (64 * QW);
+  const int set = SETS > 1 ? wave / QW : 0;
   u32x4_t *lq = lds + set * 4 * TILE, *lg = lq + 2 * TILE;
   float *ll = lsum + set * 4 * BQ, *ld = ll + 2 * BQ;
   const int k0 = t.r0 + 32 * (wave % QW), ki = k0 + (lane & 31);
   const bool ok = ki < t.len;
   const int first = a.causal ? t.r0 : 0, per = (t.len - first + BQ - 1) / BQ, n = per * group;
-  float rl = 0.f, rd = 0.f;
   int r0 = first, head = hk * group;  // the tile last loaded: query rows r0 on of a head
   JaStage<T, DP, BQ, BYTES, QW> sq, sg;
   auto next = [&]() {
@@ -166,17 +167,10 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dkv_kernel(JaggedA
   auto load = [&](int buf) {
     sq.load(ja_lds(lq + buf * TILE), SETS * BQ);
     sg.load(ja_lds(lg + buf * TILE), SETS * BQ);
-    if (tid < BQ) {
-      const int r = r0 + tid;
-      rl = r < t.len ? a.lse[head * a.rows + t.s0 + r] : INFINITY;  // no probability
-      rd = r < t.len ? a.delta[head * a.rows + t.s0 + r] : 0.f;
-    }
-  };
-  auto store = [&](int buf) {
-    if (tid < BQ) {
-      ll[buf * BQ + tid] = rl;
-      ld[buf * BQ + tid] = rd;
-    }
+    // rows past the end come as zeros in all four: their probabilities of 1 meet zeros
+    const int64_t row = head * a.rows + t.s0 + r0;
+    if (wave % QW == 0) ja_stage_floats<BQ>(a.lse + row, t.len - r0, ja_lds(ll + buf * BQ));
+    if (wave % QW == 1) ja_stage_floats<BQ>(a.delta + row, t.len - r0, ja_lds(ld + buf * BQ));
   };
   if (set < n) load(0);
   JaRows<T, DP, ja_keep<T, DP>> k, v;
@@ -188,7 +182,6 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dkv_kernel(JaggedA
     if (WANT & 2) ak[i] = f16_zero();
     if (WANT & 1) av[i] = f16_zero();
   }
-  if (set < n) store(0);
   ja_landed();
   for (int i = set, buf = 0; i - set < n; i += SETS, buf ^= 1) {
     const int now = r0;
@@ -231,7 +224,6 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dkv_kernel(JaggedA
         }
       }
     }
-    if (i + SETS < n) store(buf ^ 1);
     ja_landed();
   }
   if constexpr (SETS > 1) {
@@ -308,7 +300,10 @@ static void bwd_shape(const JaggedAttnArgs& a, hipStream_t st) {
       dq_run<T, DP, 32, BYTES, 4, 2>(a, st);
     else
       dq_run<T, DP, 32, BYTES, 4, 1>(a, st);
-    dkv_run<T, DP, 32, 3, BYTES, 2, 2>(a, st);
+    if (jagged_few(a, a.Hkv, 2.75f))
+      dkv_run<T, DP, 32, 3, BYTES, 2, 2>(a, st);
+    else
+      dkv_run<T, DP, 32, 3, BYTES, 4, 1>(a, st);
   } else {
     if (jagged_few(a, H, 1.5f))
       dq_run<T, DP, 32, BYTES, 2, 2>(a, st);
