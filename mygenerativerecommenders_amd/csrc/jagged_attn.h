@@ -523,9 +523,11 @@ constexpr bool ja_keep = sizeof(T) == 2 || DP <= 128;
 
 // Whether there are at most `per_cu` tiles of 128 rows for each CU.  The fewer the tiles, the
 // more wave sets share a workgroup's: the longest tile's time is what counts then, and with
-// many tiles the joining is only in the way.  Measured over ragged batches (us):
-//   forward / key pass, 24 x 1,499 rows, 8 heads on 2 of 64: 4 waves 45 / 176, 4 sets of two 51 / 106;
-//   2 x 8,192 rows, 4 heads of 128, forward: one set 146, two sets 109; 128 x 700: 87 and 117.
+// many tiles the joining is only in the way.  Measured over ragged batches, bf16 (us):
+//   width 64, forward / dQ / key pass: 32 x 2,028 rows, 1 head (302 tiles): 4 sets of two waves 37 / 41 / 46, one
+//   set of four 49 / 61 / 64; 24 x 1,000, 2 heads (422): 37 / 41 / 46 and 30 / 36 / 39;
+//   width 128, forward: 2 x 8,192 rows, 4 heads (392): two sets 109, one 146; 24 x 980, 4 heads (488):
+//   42 and 40; 128 x 700, 4 heads (2,000): 117 and 87.
 // Key pass at width 128: 24 x 1,000 rows, 4 heads (488 tiles): two sets 44, one 62; 128 x 996, 8 heads on
 // one (653): 275 and 406; 200 x 100, 2 heads (712): 28 and 21; 128 x 996, 4 heads (2,612): 239 and 192.
 // At width 256 a workgroup of two sets fills a CU's LDS and one of a single set half of it, and then

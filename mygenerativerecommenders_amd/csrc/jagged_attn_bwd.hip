@@ -287,16 +287,16 @@ static void bwd_shape(const JaggedAttnArgs& a, hipStream_t st) {
       dkv_run<T, DP, 32, 2, BYTES, 4, 1>(a, st);
     }
   } else if constexpr (DP == 64) {
-    if (jagged_few(a, H, 2))
+    if (jagged_few(a, H, 1.5f))
       dq_run<T, DP, 64, BYTES, 2, 4>(a, st);
     else
       dq_run<T, DP, 64, BYTES, 4, 1>(a, st);
-    if (jagged_few(a, a.Hkv, 2))
+    if (jagged_few(a, a.Hkv, 1.5f))
       dkv_run<T, DP, 32, 3, BYTES, 2, 4>(a, st);
     else
       dkv_run<T, DP, 64, 3, BYTES, 4, 1>(a, st);
   } else if constexpr (DP == 128) {
-    if (jagged_few(a, H, 2))
+    if (jagged_few(a, H, 2.f))
       dq_run<T, DP, 32, BYTES, 4, 2>(a, st);
     else
       dq_run<T, DP, 32, BYTES, 4, 1>(a, st);

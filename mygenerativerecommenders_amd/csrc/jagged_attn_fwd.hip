@@ -190,7 +190,7 @@ static void fwd_shape(const JaggedAttnArgs& a, hipStream_t st) {
       fwd_run<T, DP, 32, BYTES, 4, 1>(a, st);
     }
   } else if constexpr (DP <= 128) {
-    if (jagged_few(a, H, 2))
+    if (jagged_few(a, H, DP == 64 ? 1.5f : 2.f))
       fwd_run<T, DP, 64, BYTES, DP == 64 ? 2 : 4, DP == 64 ? 4 : 2>(a, st);
     else
       fwd_run<T, DP, 64, BYTES, 4, 1>(a, st);
