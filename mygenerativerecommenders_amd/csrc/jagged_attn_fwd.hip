@@ -3,10 +3,19 @@
 //   S = scale Q K^T over the rows of one sequence (keys j <= i where causal),
 //   O = softmax(S) V,  lse = log2 of the rows' sums for the backward pass
 //
-// One workgroup of four waves per 128 query rows and head, a wave per 32 rows.  One pass over
-// the keys in tiles held in LDS (the next tile's loads in flight in registers meanwhile), with
-// the running maximum and sum of each row: S^T = K Q^T puts a query row in a lane, so
-// maximum, sum and rescaling are lane-local but for one exchange between lane halves.
+// A workgroup per 32 QW query rows and head, a wave per 32 rows and set, SETS sets of waves that
+// take the key tiles in turn and join their sums at the end.  One pass over the keys in tiles
+// of BN held in LDS (the next tile on its way from memory meanwhile), with the running maximum
+// and sum of each row: S^T = K Q^T puts a query row in a lane, so maximum, sum and rescaling
+// are lane-local but for one exchange between lane halves.
+//
+// Bytes are no bound (q, k, v and out once: some 10 us where a launch takes 90); what is depends on
+// the tiles.  Few of them: the longest sequence's chain of tiles (2 x 8,192 rows, 4 heads of 128,
+// bf16: 137 us, 540 TFLOP/s).  Many: the vector work of the softmax, 16 exponentials a lane
+// and tile beside 16 (width 64) to 64 matrix instructions, hidden only by other waves of the
+// SIMD (128 x 996 rows, 4 heads of 128: 156 us).  Tried and slower: the next tile's scores under this
+// tile's softmax in one wave (54 us -> 71, 213 -> 246), as the registers cost it a wave; tiles staged
+// through registers.
 #include <math.h>
 
 #include "jagged_attn.h"

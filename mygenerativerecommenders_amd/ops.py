@@ -1232,7 +1232,8 @@ def jagged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     by default.  Returns (rows, H, dv) of q's type; rows before offsets[0] and from offsets[B] on are
     zero, and so are their gradients.  H dv < 2^22.  An infinity or NaN in a row can reach every
     row of its sequence and key head, those before it included, and no other.  Softmax and sums are fp32; bfloat16 probabilities enter the products
-    rounded to bfloat16.  No atomics: the same bits every run."""
+    rounded to bfloat16, with their rounding errors as a second operand where a gradient is wanted
+    (so such outputs can differ in the last bit).  No atomics: the same bits every run."""
     _lib.require_gpu(q, k, v, offsets)
     if q.dtype not in _FLOATS or k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError("jagged_attention: q, k and v must be float32 or bfloat16, all the same")
