@@ -71,6 +71,17 @@ __device__ __forceinline__ int wave_isum(int v) {
          __builtin_amdgcn_readlane(v, 48);
 }
 
+// Maximum over the wave, in every lane; values >= 0.
+__device__ __forceinline__ int wave_imax(int v) {
+  auto mov = [](int x, auto ctrl) { return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, 0xF, 0xF, true); };
+  v = max(v, mov(v, std::integral_constant<int, 0xB1>{}));
+  v = max(v, mov(v, std::integral_constant<int, 0x4E>{}));
+  v = max(v, mov(v, std::integral_constant<int, 0x141>{}));
+  v = max(v, mov(v, std::integral_constant<int, 0x140>{}));
+  return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+
 // Tile `slot` of the jagged rows in tiles of BM rows that never cross a sequence; the rows before
 // the first and past the last sequence are tiled as one more each (`none`).  The host knows neither
 // lengths nor tile counts, only that rows / BM + B + 2 slots are enough.  Offsets are clamped to
@@ -126,7 +137,8 @@ __device__ __forceinline__ JaggedTile jagged_tile(const int64_t* offsets, int B,
       t.r0 = (int)r0;
       return t;
     }
-    int n = 1, more = (int)(rows / BM) + 2, past = 0;  // level n has the slot or is below it
+    // level n has the slot or is below it, level `more` is empty or above it
+    int n = 1, more = wave_imax(max(max(tiles[0], tiles[1]), max(tiles[2], tiles[3]))) + 1, past = 0;
     while (more - n > 1) {
       const int mid = (n + more) >> 1, c = above(mid);
       if (c > slot) {
