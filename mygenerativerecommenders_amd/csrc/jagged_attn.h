@@ -40,7 +40,6 @@ struct JaggedAttnArgs {
   float* delta;      // (H, rows): sum(dout * out)
   int64_t slots;     // tiles of the rows per head, see jagged_tile
   int wide;          // rows and their starts are multiples of 16 bytes
-  int heads_per_key; // the backward's key pass: `group`, where that is 1 for its grid
 };
 
 // Work item of a workgroup: slot, key head, and query head of its group.  Workgroups i, i + 8, ..
@@ -51,8 +50,8 @@ struct JaggedWork {
   int64_t slot;  // >= slots: nothing
 };
 inline int64_t jagged_grid(int64_t slots, int Hkv, int group) { return (slots * Hkv + 7) / 8 * 8 * group; }
-__device__ __forceinline__ JaggedWork jagged_work(const JaggedAttnArgs& a, unsigned id) {
-  const unsigned group = (unsigned)a.group, j = id / 8, u = j / group * 8 + id % 8;
+__device__ __forceinline__ JaggedWork jagged_work(const JaggedAttnArgs& a, unsigned group, unsigned id) {
+  const unsigned j = id / 8, u = j / group * 8 + id % 8;
   JaggedWork k;
   k.g = (int)(j % group);
   k.slot = u / (unsigned)a.Hkv;

@@ -3,15 +3,15 @@
 // The probabilities are recomputed from the scores and the rows' log-sums, never stored:
 //   P = 2^(S scale / ln 2 - lse),  dP = dO V^T,  D = sum(dO O),  dS = P (dP - D)
 //   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO
-// Two launches, each with its result in registers and no atomics, so the bits do not depend
+// Two passes, each with its result in registers and no atomics, so the bits do not depend
 // on the order of workgroups: one over query rows (dQ, and D for the other), one over key
 // rows (dK and dV, summed over the query heads that share them).  Seven products instead
-// of the five that a single launch with atomic dQ sums would take (eight at widths above 128).
+// of the five that one pass with atomic dQ sums would take (eight at widths above 128).
 //
-// bf16, 32 x 2,059 ragged rows, one head of 256: dQ 104 us, dV 83, dK 104, one wave a SIMD and
-// bound by the longest sequence's chain of tiles.  24 x 1,499 rows, 8 heads on 2 of 64: 58 and 98.
+// bf16, 32 x 2,059 ragged rows, one head of 256: 263 us (alone dQ 104, dV 83, dK 104), one wave a
+// SIMD and bound by the longest sequence's chain of tiles.  24 x 1,499 rows, 8 heads on 2 of 64: 58 and 98.
 // 128 x 996 rows, 4 heads of 128: 201 and 195, two waves a SIMD.  fp32 runs at half the matrix rate:
-// 128 x 211 rows, one head of 50: 25 and 31, of which some 11 each are what one tile takes.
+// 128 x 211 ragged rows, one head of 50: 46 us, of which some 16 are what one tile takes.
 #include <math.h>
 
 #include "jagged_attn.h"
@@ -21,14 +21,14 @@
 namespace gr {
 
 // dQ: a workgroup per 32 QW query rows and head, a wave per 32 rows and set, tiles of BN keys.
-template <typename T, int DP, int BN, int BYTES, int QW, int SETS>
-__global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dq_kernel(JaggedAttnArgs a) {
+// GIVEN: D is in `delta` already.
+template <typename T, int DP, int BN, int BYTES, int QW, int SETS, bool GIVEN>
+__device__ __forceinline__ void ja_dq(const JaggedAttnArgs& a, unsigned block, u32x4_t* lds) {
   using F = JaFrag<T>;
   using Tile = JaTile<T, DP>;
   constexpr int BM = 32 * QW, NB = BN / 32, DT = DP / 32, TILE = Tile::size(BN);
-  __shared__ u32x4_t lds[SETS * 4 * TILE];
-  static_assert(sizeof(lds) >= (SETS - 1) * QW * DT * 16 * 256, "the other sets' sums fit");
-  const JaggedWork wk = jagged_work(a, blockIdx.x);
+  static_assert(SETS * 4 * TILE * 16 >= (SETS - 1) * QW * DT * 16 * 256, "the other sets' sums fit");
+  const JaggedWork wk = jagged_work(a, a.group, block);
   if (wk.slot >= a.slots) return;
   const int head = wk.hk * a.group + wk.g, H = a.Hkv * a.group;
   const JaggedTile t = jagged_tile<BM, false>(a.offsets, a.B, a.rows, wk.slot);
@@ -59,8 +59,11 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dq_kernel(JaggedAt
   q.init((const T*)a.q + t.s0 * a.ld_q + head * a.hs_q, a.ld_q, q0, t.len, a.d);
   const int64_t out0 = (t.s0 * H + head) * a.dv;
   go.init((const T*)a.dout + out0, (int64_t)H * a.dv, q0, t.len, a.dv);
+  const int64_t at = head * a.rows + t.s0 + (ok ? qi : 0);
   float delta = 0.f;
-  {
+  if constexpr (GIVEN) {
+    delta = a.delta[at];
+  } else {
     JaRows<T, DP, false> out, low;
     out.init((const T*)a.out + out0, (int64_t)H * a.dv, q0, t.len, a.dv);
     low.init((const T*)(sizeof(T) == 2 ? a.out_low : a.out) + out0, (int64_t)H * a.dv, q0, t.len, a.dv);
@@ -74,9 +77,8 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dq_kernel(JaggedAt
       for (int i = 0; i < 16 / (int)sizeof(T); ++i) delta += (sizeof(T) == 2 ? x[i] + z[i] : x[i]) * y[i];
     }
     delta = half_sum(delta);
+    if (ok && half == 0 && set == 0) a.delta[at] = delta;
   }
-  const int64_t at = head * a.rows + t.s0 + (ok ? qi : 0);
-  if (ok && half == 0 && set == 0) a.delta[at] = delta;
   const float lse = ok ? a.lse[at] : INFINITY;
   f32x16 acc[DT];
 #pragma unroll
@@ -125,16 +127,14 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dq_kernel(JaggedAt
 // where the compiler is held to it (not with two sets and loads of 4 bytes, whose lanes have more
 // addresses): 128 sequences of up to 996 rows, 4 heads, 334 us -> 192.
 template <typename T, int DP, int BQ, int WANT, int BYTES, int QW, int SETS>
-__global__ __launch_bounds__(64 * QW * SETS, sizeof(T) == 2 && DP == 128 && (BYTES == 16 || SETS == 1) ? 2 : 1) void jagged_attn_dkv_kernel(JaggedAttnArgs a) {
+__device__ __forceinline__ void ja_dkv(const JaggedAttnArgs& a, unsigned block, u32x4_t* lds, float* lsum) {
   using F = JaFrag<T>;
   using Tile = JaTile<T, DP>;
   constexpr int BM = 32 * QW, NB = BQ / 32, DT = DP / 32, TILE = Tile::size(BQ);
-  __shared__ u32x4_t lds[SETS * 4 * TILE];
-  __shared__ __attribute__((aligned(16))) float lsum[SETS * 4 * BQ];
-  static_assert(sizeof(lds) >= (SETS - 1) * QW * DT * 16 * 256, "the other sets' sums fit");
-  const JaggedWork wk = jagged_work(a, blockIdx.x);
-  if (wk.slot >= a.slots) return;  // group 1: an item per key head
-  const int hk = wk.hk, group = a.heads_per_key, H = a.Hkv * group;
+  static_assert(SETS * 4 * TILE * 16 >= (SETS - 1) * QW * DT * 16 * 256, "the other sets' sums fit");
+  const JaggedWork wk = jagged_work(a, 1, block);  // an item per key head
+  if (wk.slot >= a.slots) return;
+  const int hk = wk.hk, group = a.group, H = a.Hkv * group;
   const JaggedTile t = jagged_tile<BM, true>(a.offsets, a.B, a.rows, wk.slot);
   if (t.len == 0) return;
   T* dk = (T*)a.dk + ((t.s0 + t.r0) * a.Hkv + hk) * a.d;
@@ -257,6 +257,66 @@ __global__ __launch_bounds__(64 * QW * SETS, sizeof(T) == 2 && DP == 128 && (BYT
 }
 
 template <typename T, int DP, int BN, int BYTES, int QW, int SETS>
+__global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_dq_kernel(JaggedAttnArgs a) {
+  __shared__ u32x4_t lds[SETS * 4 * JaTile<T, DP>::size(BN)];
+  ja_dq<T, DP, BN, BYTES, QW, SETS, false>(a, blockIdx.x, lds);
+}
+template <typename T, int DP, int BQ, int WANT, int BYTES, int QW, int SETS>
+__global__ __launch_bounds__(64 * QW * SETS, sizeof(T) == 2 && DP == 128 && (BYTES == 16 || SETS == 1) ? 2 : 1)
+    void jagged_attn_dkv_kernel(JaggedAttnArgs a) {
+  __shared__ u32x4_t lds[SETS * 4 * JaTile<T, DP>::size(BQ)];
+  __shared__ __attribute__((aligned(16))) float lsum[SETS * 4 * BQ];
+  ja_dkv<T, DP, BQ, WANT, BYTES, QW, SETS>(a, blockIdx.x, lds, lsum);
+}
+
+// Few tiles: all passes in one launch, the key rows' workgroups first, after a launch for D.
+// Alone, each leaves CUs idle behind its longest tiles; with many, a pass would only have the
+// other's registers.  `keys` workgroups for each key pass.  In turn and joint (us), fp32 width 64:
+// 4 x 1,762 rows, 4 heads (144 tiles of 128 rows) 219 and 129, 128 x 211, 1 head (339) 62 and 55, 200 x 100,
+// 2 heads (712) 70 and 65; bf16 width 64: 32 x 2,028, 1 head (302) 82 and 74, 24 x 980, 4 heads (488)
+// 70 and 74; width 128: 144 tiles 102 and 60, 282 tiles 74 and 80; width 256: 144 tiles 214 and 147,
+// 302 274 and 263, 488 234 and 242.
+template <typename T, int DP, int BN, int BYTES, int QW, int SETS>
+__global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_both_kernel(JaggedAttnArgs a, unsigned keys) {
+  __shared__ u32x4_t lds[SETS * 4 * JaTile<T, DP>::size(BN)];
+  __shared__ __attribute__((aligned(16))) float lsum[SETS * 4 * BN];
+  if constexpr (DP <= 128) {
+    if (blockIdx.x < keys)
+      ja_dkv<T, DP, BN, 3, BYTES, QW, SETS>(a, blockIdx.x, lds, lsum);
+    else
+      ja_dq<T, DP, BN, BYTES, QW, SETS, true>(a, blockIdx.x - keys, lds);
+  } else {
+    if (blockIdx.x < keys)
+      ja_dkv<T, DP, BN, 2, BYTES, QW, SETS>(a, blockIdx.x, lds, lsum);
+    else if (blockIdx.x < 2 * keys)
+      ja_dkv<T, DP, BN, 1, BYTES, QW, SETS>(a, blockIdx.x - keys, lds, lsum);
+    else
+      ja_dq<T, DP, BN, BYTES, QW, SETS, true>(a, blockIdx.x - 2 * keys, lds);
+  }
+}
+
+// D: 16 lanes for each row and head.
+template <typename T>
+__global__ __launch_bounds__(256) void jagged_attn_delta_kernel(JaggedAttnArgs a) {
+  const int64_t H = (int64_t)a.Hkv * a.group, i = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;  // row * H + head
+  if (i >= a.rows * H) return;
+  const T *o = (const T*)a.out + i * a.dv, *e = sizeof(T) == 2 ? (const T*)a.out_low + i * a.dv : nullptr,
+          *g = (const T*)a.dout + i * a.dv;
+  float s = 0.f;
+  for (int c = threadIdx.x % 16; c < a.dv; c += 16) s += ((float)o[c] + (e ? (float)e[c] : 0.f)) * (float)g[c];
+  s = sum16(s);
+  if (threadIdx.x % 16 == 0) a.delta[i % H * a.rows + i / H] = s;
+}
+
+template <typename T, int DP, int BN, int BYTES, int QW, int SETS>
+static void both_run(JaggedAttnArgs a, hipStream_t st) {
+  a.slots = jagged_slots(a.rows, a.B, 32 * QW);
+  const int64_t keys = jagged_grid(a.slots, a.Hkv, 1);
+  hipLaunchKernelGGL((jagged_attn_delta_kernel<T>), dim3((unsigned)((a.rows * a.Hkv * a.group + 15) / 16)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((jagged_attn_both_kernel<T, DP, BN, BYTES, QW, SETS>),
+                     dim3((unsigned)(keys * (DP <= 128 ? 1 : 2) + jagged_grid(a.slots, a.Hkv, a.group))), dim3(64 * QW * SETS), 0, st, a, (unsigned)keys);
+}
+template <typename T, int DP, int BN, int BYTES, int QW, int SETS>
 static void dq_run(JaggedAttnArgs a, hipStream_t st) {
   a.slots = jagged_slots(a.rows, a.B, 32 * QW);
   hipLaunchKernelGGL((jagged_attn_dq_kernel<T, DP, BN, BYTES, QW, SETS>), dim3((unsigned)jagged_grid(a.slots, a.Hkv, a.group)),
@@ -265,8 +325,6 @@ static void dq_run(JaggedAttnArgs a, hipStream_t st) {
 template <typename T, int DP, int BQ, int WANT, int BYTES, int QW, int SETS>
 static void dkv_run(JaggedAttnArgs a, hipStream_t st) {
   a.slots = jagged_slots(a.rows, a.B, 32 * QW);
-  a.heads_per_key = a.group;
-  a.group = 1;
   hipLaunchKernelGGL((jagged_attn_dkv_kernel<T, DP, BQ, WANT, BYTES, QW, SETS>), dim3((unsigned)jagged_grid(a.slots, a.Hkv, 1)),
                      dim3(64 * QW * SETS), 0, st, a);
 }
@@ -276,50 +334,63 @@ static void bwd_shape(const JaggedAttnArgs& a, hipStream_t st) {
   if constexpr (sizeof(T) == 4) {
     if constexpr (DP == 64) {
       if (jagged_few(a, H, 1))
-        dq_run<T, DP, 32, BYTES, 2, 4>(a, st);
-      else
+        both_run<T, DP, 32, BYTES, 2, 4>(a, st);
+      else if (jagged_few(a, H, 3))
+        both_run<T, DP, 32, BYTES, 2, 2>(a, st);
+      else {
         dq_run<T, DP, 32, BYTES, 2, 2>(a, st);
-      if (jagged_few(a, a.Hkv, 1))
-        dkv_run<T, DP, 32, 3, BYTES, 2, 4>(a, st);
-      else
-        dkv_run<T, DP, 32, 3, BYTES, 2, 2>(a, st);
+        if (jagged_few(a, a.Hkv, 1))
+          dkv_run<T, DP, 32, 3, BYTES, 2, 4>(a, st);
+        else
+          dkv_run<T, DP, 32, 3, BYTES, 2, 2>(a, st);
+      }
     } else if constexpr (DP == 128) {
+      if (jagged_few(a, H, 3)) return both_run<T, DP, 32, BYTES, 2, 2>(a, st);
       dq_run<T, DP, 32, BYTES, 2, 2>(a, st);
       dkv_run<T, DP, 32, 3, BYTES, 2, 2>(a, st);
     } else {
+      // (the joint kernel does not fit the scalar registers)
       dq_run<T, DP, 32, BYTES, 4, 1>(a, st);
       dkv_run<T, DP, 32, 1, BYTES, 4, 1>(a, st);
       dkv_run<T, DP, 32, 2, BYTES, 4, 1>(a, st);
     }
-  } else if constexpr (DP == 64) {
-    if (jagged_few(a, H, 1.5f))
-      dq_run<T, DP, 64, BYTES, 2, 4>(a, st);
-    else
-      dq_run<T, DP, 64, BYTES, 4, 1>(a, st);
-    if (jagged_few(a, a.Hkv, 1.5f))
-      dkv_run<T, DP, 32, 3, BYTES, 2, 4>(a, st);
-    else
-      dkv_run<T, DP, 64, 3, BYTES, 4, 1>(a, st);
-  } else if constexpr (DP == 128) {
-    if (jagged_few(a, H, 2.f))
-      dq_run<T, DP, 32, BYTES, 4, 2>(a, st);
-    else
-      dq_run<T, DP, 32, BYTES, 4, 1>(a, st);
-    if (jagged_few(a, a.Hkv, 2.75f))
-      dkv_run<T, DP, 32, 3, BYTES, 2, 2>(a, st);
-    else
-      dkv_run<T, DP, 32, 3, BYTES, 4, 1>(a, st);
+    return;
   } else {
-    if (jagged_few(a, H, 1.5f))
-      dq_run<T, DP, 32, BYTES, 2, 2>(a, st);
-    else
-      dq_run<T, DP, 32, BYTES, 4, 1>(a, st);
-    if (jagged_few(a, a.Hkv, 1.5f)) {
-      dkv_run<T, DP, 32, 1, BYTES, 2, 2>(a, st);
-      dkv_run<T, DP, 32, 2, BYTES, 2, 2>(a, st);
+    // (with loads of 4 bytes the joint kernel's addresses do not fit the scalar registers)
+    if constexpr (BYTES == 16) {
+      if (jagged_few(a, H, DP == 128 ? 1.f : 1.5f))
+        return both_run<T, DP, 32, BYTES, 2, DP == 64 ? 4 : 2>(a, st);
+    }
+    if constexpr (DP == 64) {
+      if (BYTES == 4 && jagged_few(a, H, 1.5f))
+        dq_run<T, DP, 64, 4, 2, 4>(a, st);
+      else
+        dq_run<T, DP, 64, BYTES, 4, 1>(a, st);
+      if (jagged_few(a, a.Hkv, 1.5f))
+        dkv_run<T, DP, 32, 3, BYTES, 2, 4>(a, st);
+      else
+        dkv_run<T, DP, 64, 3, BYTES, 4, 1>(a, st);
+    } else if constexpr (DP == 128) {
+      if (jagged_few(a, H, 2.f))
+        dq_run<T, DP, 32, BYTES, 4, 2>(a, st);
+      else
+        dq_run<T, DP, 32, BYTES, 4, 1>(a, st);
+      if (jagged_few(a, a.Hkv, 2.75f))
+        dkv_run<T, DP, 32, 3, BYTES, 2, 2>(a, st);
+      else
+        dkv_run<T, DP, 32, 3, BYTES, 4, 1>(a, st);
     } else {
-      dkv_run<T, DP, 32, 1, BYTES, 4, 1>(a, st);
-      dkv_run<T, DP, 32, 2, BYTES, 4, 1>(a, st);
+      if (BYTES == 4 && jagged_few(a, H, 1.5f))
+        dq_run<T, DP, 32, 4, 2, 2>(a, st);
+      else
+        dq_run<T, DP, 32, BYTES, 4, 1>(a, st);
+      if (jagged_few(a, a.Hkv, 1.5f)) {
+        dkv_run<T, DP, 32, 1, BYTES, 2, 2>(a, st);
+        dkv_run<T, DP, 32, 2, BYTES, 2, 2>(a, st);
+      } else {
+        dkv_run<T, DP, 32, 1, BYTES, 4, 1>(a, st);
+        dkv_run<T, DP, 32, 2, BYTES, 4, 1>(a, st);
+      }
     }
   }
 }

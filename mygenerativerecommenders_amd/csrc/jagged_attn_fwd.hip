@@ -34,7 +34,7 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedA
   constexpr int BM = 32 * QW, NB = BN / 32, DT = DP / 32, TILE = Tile::size(BN);
   __shared__ u32x4_t lds[SETS * 4 * TILE];
   static_assert(sizeof(lds) >= (SETS - 1) * (QW * DT * 16 + 2 * QW) * 256, "the other sets' sums fit");
-  const JaggedWork wk = jagged_work(a, blockIdx.x);
+  const JaggedWork wk = jagged_work(a, a.group, blockIdx.x);
   if (wk.slot >= a.slots) return;
   const int head = wk.hk * a.group + wk.g, H = a.Hkv * a.group;
   const JaggedTile t = jagged_tile<BM, false>(a.offsets, a.B, a.rows, wk.slot);
