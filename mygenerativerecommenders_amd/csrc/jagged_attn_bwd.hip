@@ -300,10 +300,16 @@ template <typename T>
 __global__ __launch_bounds__(256) void jagged_attn_delta_kernel(JaggedAttnArgs a) {
   const int64_t H = (int64_t)a.Hkv * a.group, i = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;  // row * H + head
   if (i >= a.rows * H) return;
-  const T *o = (const T*)a.out + i * a.dv, *e = sizeof(T) == 2 ? (const T*)a.out_low + i * a.dv : nullptr,
-          *g = (const T*)a.dout + i * a.dv;
+  constexpr int V = 16 / sizeof(T);
   float s = 0.f;
-  for (int c = threadIdx.x % 16; c < a.dv; c += 16) s += ((float)o[c] + (e ? (float)e[c] : 0.f)) * (float)g[c];
+  for (int c = threadIdx.x % 16 * V; c < a.dv; c += 16 * V) {
+    float x[V], y[V], z[V];
+    ja_floats<T>(ja_fix16<T>(ja_load16<T>((const T*)a.out + i * a.dv, c, a.dv), c, a.dv), x);
+    ja_floats<T>(ja_fix16<T>(ja_load16<T>((const T*)a.dout + i * a.dv, c, a.dv), c, a.dv), y);
+    if (sizeof(T) == 2) ja_floats<T>(ja_fix16<T>(ja_load16<T>((const T*)a.out_low + i * a.dv, c, a.dv), c, a.dv), z);
+#pragma unroll
+    for (int j = 0; j < V; ++j) s += (sizeof(T) == 2 ? x[j] + z[j] : x[j]) * y[j];
+  }
   s = sum16(s);
   if (threadIdx.x % 16 == 0) a.delta[i % H * a.rows + i / H] = s;
 }
