@@ -92,7 +92,8 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedA
       // summed stays below 2^8 times the rows, and the rescaling is rare.
       if (__builtin_expect(__any((top - m) * a.scale_l2 > 8.f), 0)) {
         top = fmaxf(top, m);
-        const float f = __builtin_amdgcn_exp2f((m - top) * a.scale_l2);
+        // rows that have met nothing but -inf are asked too where another row of the wave runs ahead
+        const float f = m == top ? 1.f : __builtin_amdgcn_exp2f((m - top) * a.scale_l2);
         m = top;
         l *= f;
 #pragma unroll

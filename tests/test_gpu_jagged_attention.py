@@ -360,3 +360,26 @@ def test_empty_batches():
     some = torch.randn(9, 2, 16, device="cuda")
     for offsets in (torch.zeros(1, dtype=torch.int64, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")):
         assert (ops.jagged_attention(some, some, some, offsets) == 0).all()
+
+
+@DTYPES
+@pytest.mark.parametrize("d", [40, 128, 256])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+def test_one_row_of_a_wave_overflows_to_minus_infinity(causal, d, dtype):
+    """Scores of a few rows overflow to -inf over the first tiles, their neighbours' are ordinary: the
+    rows' sums are those of the keys behind, where all their scores are zero."""
+    n, first = 300, 140
+    _, _, v, offsets, dout = make([n], 1, 1, d, d, dtype)
+    q, k = torch.full((n, 1, d), 1e-25, device="cuda").to(dtype), torch.zeros(n, 1, d, device="cuda").to(dtype)
+    k[:first] = -1e25
+    q[first + 3::37] = 1e30
+    S = d ** -0.5 * (q[:, 0].double() @ k[:, 0].double().T)
+    S[S < -1e30] = -math.inf
+    if causal:
+        S = S.masked_fill(~torch.ones(n, n, dtype=torch.bool, device="cuda").tril(), -math.inf)
+    err = 2 * (d + 2) * U * d ** 0.5 + (8 + n + 2 * d ** 0.5) * U  # |q k| sums to d
+    P, V, b = torch.softmax(S, -1), v[:, 0].double(), 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+    lim = (err + b + n * U) * (P @ V.abs()) + (b + 4 * U) * (P @ V).abs() + 1e-30
+    out, *grads = run(q, k, v, offsets, dout, causal=causal)
+    assert ((out[:, 0].double() - P @ V).abs() <= lim).all()
+    assert all(torch.isfinite(t).all() for t in grads)
