@@ -325,7 +325,8 @@ GR_API int gr_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64
  * before offsets[0] and from offsets[B] on get zeros and are not read; offsets are clamped to
  * [0, rows].  An infinity or NaN in a row can reach every row of its sequence and key head, those
  * before it included, and no other.  lse (H, rows): log2 of each row's
- * sum of exp(scaled scores); out_low (bf16 only, as out): what rounding left off out, so that
+ * sum of exp(scaled scores), +inf where the largest of them is beyond 2^23 ln 2 in magnitude (such a row
+ * gives no gradient); out_low (bf16 only, as out): what rounding left off out, so that
  * the backward's sum(dout out) is that of the unrounded rows.  The backward needs both
  * (forward: NULL if there is none).
  * The backward recomputes the probabilities; dk / dvv sum over the heads that share them.

@@ -32,7 +32,7 @@ struct JaggedAttnArgs {
   float scale_l2;  // scale / ln 2
   void* out;       // (rows, H, dv)
   void* out_low;   // bf16: what out's rounding left off, or NULL
-  float* lse;      // (H, rows): log2 of each row's sum of 2^(scaled score / ln 2), or NULL
+  float* lse;      // (H, rows): log2 of each row's sum of 2^(scaled score / ln 2), +inf from 2^23 on, or NULL
   const void* dout;  // (rows, H, dv)
   void* dq;          // (rows, H, d)
   void* dk;          // (rows, Hkv, d)

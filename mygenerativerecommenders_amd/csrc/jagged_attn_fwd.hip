@@ -66,6 +66,9 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedA
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = f16_zero();
   float m = -INFINITY, l = 0.f;
+  // Whether a row of the wave has a maximum so far from zero that m * scale_l2, rounded, is off by
+  // more than a term can be (keys masked by a type's lowest value): the difference is taken first then.
+  bool far = false;
   // every set makes the same number of rounds, the last one perhaps without a tile
   for (int k0 = first, buf = 0; k0 - first < keys; k0 += step, buf = TILE - buf) {
     if (k0 + step < keys) load(TILE - buf);
@@ -98,8 +101,16 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedA
         l *= f;
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[i] *= f;
+        far = __any(m > -INFINITY && fabsf(m) * a.scale_l2 > 0x1p20f);
       }
-      const float mc = m == -INFINITY ? 0.f : m * a.scale_l2;  // nothing but -inf so far: no terms
+      float mc = m == -INFINITY ? 0.f : m * a.scale_l2;  // nothing but -inf so far: no terms
+      if (__builtin_expect(far, 0)) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[b][r] -= m == -INFINITY ? 0.f : m;
+        mc = 0.f;
+      }
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -149,7 +160,11 @@ __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_fwd_kernel(JaggedA
   const float inv = 1.f / l;
 #pragma unroll
   for (int i = 0; i < DT; ++i) ja_store_t<T>((T*)a.out + out0, 32 * i, a.dv, o[i], inv, ok, low);
-  if (a.lse && ok && half == 0) a.lse[head * a.rows + t.s0 + qi] = m * a.scale_l2 + __builtin_amdgcn_logf(l);
+  // From 2^23 on a log-sum does not hold the sum any more, and the backward pass could not tell such a
+  // row's probabilities: +inf makes them zero.
+  if (a.lse && ok && half == 0)
+    a.lse[head * a.rows + t.s0 + qi] =
+        m > -INFINITY && fabsf(m * a.scale_l2) > 0x1p23f ? INFINITY : m * a.scale_l2 + __builtin_amdgcn_logf(l);
 }
 
 int jagged_attn_check(const char* what, JaggedAttnArgs& a, int H, int bf16) {

@@ -1231,7 +1231,10 @@ def jagged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     stride, so column slices of one projection are read in place.  ``scale`` > 0, 1 / sqrt(d)
     by default.  Returns (rows, H, dv) of q's type; rows before offsets[0] and from offsets[B] on are
     zero, and so are their gradients.  H dv < 2^22.  An infinity or NaN in a row can reach every
-    row of its sequence and key head, those before it included, and no other.  Softmax and sums are fp32; bfloat16 probabilities enter the products
+    row of its sequence and key head, those before it included, and no other.  Keys masked by a lowest
+    value in a column of theirs are no part of a row that sees another key; a row whose largest scaled
+    score is beyond 5.8e6 in magnitude (it sees masked keys alone, say) gives no gradient: its log-sum does
+    not hold in fp32.  Softmax and sums are fp32; bfloat16 probabilities enter the products
     rounded to bfloat16, with their rounding errors as a second operand where a gradient is wanted
     (so such outputs can differ in the last bit).  No atomics: the same bits every run."""
     _lib.require_gpu(q, k, v, offsets)

@@ -383,3 +383,45 @@ def test_one_row_of_a_wave_overflows_to_minus_infinity(causal, d, dtype):
     out, *grads = run(q, k, v, offsets, dout, causal=causal)
     assert ((out[:, 0].double() - P @ V).abs() <= lim).all()
     assert all(torch.isfinite(t).all() for t in grads)
+
+
+@DTYPES
+@pytest.mark.parametrize("d", [1, 40, 128, 256])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+def test_keys_masked_by_the_lowest_value(causal, d, dtype):
+    """A column of ones in q against the type's lowest value in some keys' rows, tiles of them in the
+    front: no part of the sums of rows that see another key, forward and backward.  Rows that see no other
+    are the mean of what they see, and give no gradient."""
+    n = 330
+    q, k, v, offsets, dout = make([n], 1, 1, d, d, dtype)
+    q, k, dout = q.clone(), k.clone(), dout.clone()
+    masked = torch.zeros(n, dtype=torch.bool, device="cuda")
+    masked[:150] = masked[200:203] = masked[250:] = True
+    q[:, 0, -1] = 1
+    k[:, 0, -1] = torch.where(masked, torch.finfo(dtype).min, 0)
+    got = run(q, k, v, offsets, dout, causal=causal)
+    live = ~masked if not causal else ~masked & torch.ones(n, n, dtype=torch.bool, device="cuda").tril()
+    some = live.expand(n, n).any(1)
+    # the same rows with the masked keys' values out of the way: their probabilities are zero
+    k0 = k.clone()
+    k0[masked, 0, -1] = 0
+    b, s = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0, d ** -0.5
+    Q, K, V, G = (t[:, 0].double() for t in (q, k0, v, dout))
+    G = G * some[:, None]
+    S = s * (Q @ K.T)
+    err = (d + 2) * U * s * (Q.abs() @ K.abs().T)
+    S = S.masked_fill(~live, -math.inf)
+    seen = torch.ones(n, n, dtype=torch.float64, device="cuda")
+    seen = (seen.tril() if causal else seen) / (torch.arange(1, n + 1, device="cuda")[:, None] if causal else n)
+    P = torch.where(some[:, None], torch.softmax(S, -1), seen)
+    r = err + err.amax(1, keepdim=True) + (8 + n + 2 * S.masked_fill(~live, 0).abs().amax(1, keepdim=True)) * U
+    O, dP = P @ V, G @ V.T
+    eO = (P * (r + b + n * U)) @ V.abs()
+    D = (G * O).sum(1, keepdim=True)
+    eD = ((b + d * U) * (G * O).abs() + G.abs() * eO).sum(1, keepdim=True)
+    dS = P * (dP - D)
+    eS = r * dS.abs() + P * (eD + d * U * (G.abs() @ V.abs().T)) + (b + n * U) * dS.abs()
+    ref = [(O, eO), (s * (dS @ K), s * (eS @ K.abs())), (s * (dS.T @ Q), s * (eS.T @ Q.abs())),
+           (P.T @ G, (P * (r + b + n * U)).T @ G.abs())]
+    for name, x, (y, e) in zip(("out", "dq", "dk", "dv"), got, ref):
+        assert ((x[:, 0].double() - y).abs() <= e + (b + 4 * U) * y.abs() + 1e-30).all(), name
