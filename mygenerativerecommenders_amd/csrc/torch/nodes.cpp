@@ -127,13 +127,18 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
 }
 
 // ---------------------------------------------------------------- jagged attention
+// bfloat16 rows are read as pairs: from a start on a 4-byte boundary on
+bool pairs(const Tensor& x) { return !is16(x) || (uintptr_t)x.data_ptr() % 4 == 0; }
+// (not contiguous(), which returns what torch counts as contiguous wherever it starts, and with any
+// stride where a size is 1)
+Tensor copied(const Tensor& x) { return plain(x).copy_(x); }
 // x itself where the kernels read it in place: contiguous columns, row strides below 2^22, for
 // bfloat16 even strides and a start on a 4-byte boundary; else a contiguous copy
 Tensor columns(const Tensor& x) {
   const int64_t s0 = x.stride(0), s1 = x.stride(1);
-  bool ok = x.stride(2) == 1 && s0 >= 0 && s0 < (1 << 22);
-  if (is16(x)) ok = ok && s0 % 2 == 0 && s1 % 2 == 0 && (uintptr_t)x.data_ptr() % 4 == 0;
-  return ok ? x : x.contiguous();
+  bool ok = x.stride(2) == 1 && s0 >= 0 && s0 < (1 << 22) && pairs(x);
+  if (is16(x)) ok = ok && s0 % 2 == 0 && s1 % 2 == 0;
+  return ok ? x : copied(x);
 }
 
 Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& offsets, bool causal, double scale,
@@ -170,7 +175,7 @@ struct JaggedAttention : torch::autograd::Function<JaggedAttention> {
     {
       const at::NoGradGuard off;
       const c10::DeviceGuard guard(q.device());
-      const Tensor dout = grads[0].contiguous();
+      const Tensor dout = grads[0].is_contiguous() && pairs(grads[0]) ? grads[0] : copied(grads[0]);
       for (int i = 0; i < 3; ++i) got[i] = plain(saved[i]);
       const int64_t rows = q.size(0), h = q.size(1);
       const size_t n = e.jagged_attn_bwd_workspace_size(rows, (int)h);

@@ -425,3 +425,43 @@ def test_keys_masked_by_the_lowest_value(causal, d, dtype):
            (P.T @ G, (P * (r + b + n * U)).T @ G.abs())]
     for name, x, (y, e) in zip(("out", "dq", "dk", "dv"), got, ref):
         assert ((x[:, 0].double() - y).abs() <= e + (b + 4 * U) * y.abs() + 1e-30).all(), name
+
+
+@DTYPES
+def test_contiguous_views_that_start_anywhere(dtype):
+    """What torch counts as contiguous and the kernels' 4-byte loads do not take: an odd first element,
+    one head with a stride of its own, a single row far from the next."""
+    from mygenerativerecommenders_amd import ops
+    q, k, v, offsets, dout = make([77, 30], 4, 2, 40, 40, dtype)
+    want = run(q, k, v, offsets, dout)
+
+    def odd(t):
+        room = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        got = room[1:].view(t.shape)
+        return got.copy_(t)
+
+    for i in range(3):
+        args = [q, k, v]
+        args[i] = odd(args[i])
+        assert args[i].is_contiguous() and args[i].data_ptr() % 4 == (2 if dtype == torch.bfloat16 else 0)
+        for x, y in zip(run(*args, offsets, dout), want):
+            assert torch.equal(x, y)
+    for x, y in zip(run(q, k, v, offsets, odd(dout)), want):
+        assert torch.equal(x, y)
+    # a gradient that autograd cuts out of a longer one
+    q1, k1, v1 = (t.detach().requires_grad_(True) for t in (q, k, v))
+    out = ops.jagged_attention(q1, k1, v1, offsets)
+    joined = torch.cat([torch.zeros(3, dtype=dtype, device="cuda"), out.flatten()])
+    for x, y in zip(torch.autograd.grad(joined, (q1, k1, v1), torch.cat([torch.ones_like(joined[:3]), dout.flatten()])), want[1:]):
+        assert torch.equal(x, y)
+    # one head: its stride is 1
+    args = make([50, 13], 1, 1, 40, 40, dtype)
+    heads = [t.reshape(63, 40, 1).permute(0, 2, 1) for t in args[:3]]
+    assert heads[0].stride(1) == 1
+    for x, y in zip(run(*heads, *args[3:]), run(*args)):
+        assert torch.equal(x, y)
+    # a row of rows 2^22 apart
+    one = [t.as_strided(t[:1].shape, ((1 << 22) + 1, *t.stride()[1:])) for t in (q, k, v)]
+    ends = torch.tensor([0, 1], device="cuda")
+    for x, y in zip(run(*one, ends, dout[:1]), run(*(t[:1].clone() for t in (q, k, v)), ends, dout[:1])):
+        assert torch.equal(x, y)
