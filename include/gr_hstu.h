@@ -320,7 +320,8 @@ GR_API int gr_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64
  * q (rows, H, d), k (rows, Hkv, d), v (rows, Hkv, dv): bf16 (bf16 != 0) or fp32, element
  * strides ld_* of a row (in [0, 2^22)) and hs_* of a head, columns contiguous, no alignment
  * beyond the element's for fp32, even strides and widths from 4-byte boundaries on for bf16;
- * 16 bytes <= d, dv <= 256 elements, H a multiple of Hkv, H dv < 2^22, scale > 0.  out, dout (rows, H, dv), dq
+ * 16 bytes <= d, dv <= 256 elements, H a multiple of Hkv, H dv < 2^22, scale > 0.  The backward takes
+ * ld_q >= d only.  out, dout (rows, H, dv), dq
  * (rows, H, d), dk (rows, Hkv, d), dvv (rows, Hkv, dv) are contiguous.  offsets ascend; rows
  * before offsets[0] and from offsets[B] on get zeros and are not read; offsets are clamped to
  * [0, rows].  An infinity or NaN in a row can reach every row of its sequence and key head, those

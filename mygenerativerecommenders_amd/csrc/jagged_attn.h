@@ -234,8 +234,9 @@ struct JaTile {
 // memory (buffer loads to LDS of BYTES a lane: 16 where rows and their starts are multiples of
 // that, else 4).  They are issued where the compiler does not see them, so that it does not
 // wait for them at the next LDS read: ja_landed() waits and meets the other waves.  The
-// descriptor ends with the sequence's last row, so rows past it come as zeros, and lanes past
-// column d ask for what is out of its range.
+// descriptor ends with the sequence's last row, so rows past it come as zeros where the stride is
+// d or more (below, as rows of the sequence: only callers that mask by index take such), and lanes
+// past column d ask for what is out of its range.
 template <typename T, int DP, int R, int BYTES, int QW>
 struct JaStage {
   using Tile = JaTile<T, DP>;

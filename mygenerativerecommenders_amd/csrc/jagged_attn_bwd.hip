@@ -172,7 +172,8 @@ __device__ __forceinline__ void ja_dkv(const JaggedAttnArgs& a, unsigned block, 
   auto load = [&](int buf) {
     sq.load(ja_lds(lq + buf * TILE), SETS * BQ);
     sg.load(ja_lds(lg + buf * TILE), SETS * BQ);
-    // rows past the end come as zeros in all four: their probabilities of 1 meet zeros
+    // rows past the end come as zeros in all four (query rows are d apart at least, or the descriptor
+    // would not end before them): their probabilities of 1 meet zeros
     const int64_t row = head * a.rows + t.s0 + r0;
     if (wave % QW == 0) ja_stage_floats<BQ>(a.lse + row, t.len - r0, ja_lds(ll + buf * BQ));
     if (wave % QW == 1) ja_stage_floats<BQ>(a.delta + row, t.len - r0, ja_lds(ld + buf * BQ));
@@ -439,6 +440,7 @@ int gr_jagged_attn_bwd(const void* q, int64_t ld_q, int64_t hs_q, const void* k,
   a.dout = dout; a.dq = dq; a.dk = dk; a.dvv = dvv; a.delta = (float*)workspace;
   if (gr::jagged_attn_check("gr_jagged_attn_bwd", a, H, bf16)) return 1;
   if (rows == 0) return 0;
+  GR_REQUIRE(ld_q >= d, "gr_jagged_attn_bwd: query rows closer than their width");
   GR_REQUIRE(lse && dout && (out_low || !bf16) && dq && dk && dvv, "gr_jagged_attn_bwd: null pointer");
   GR_REQUIRE(workspace && ws_bytes >= gr_jagged_attn_bwd_workspace_size(rows, H), "gr_jagged_attn_bwd: workspace too small");
   const hipStream_t st = (hipStream_t)stream;

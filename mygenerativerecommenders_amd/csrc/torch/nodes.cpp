@@ -133,10 +133,11 @@ bool pairs(const Tensor& x) { return !is16(x) || (uintptr_t)x.data_ptr() % 4 == 
 // stride where a size is 1)
 Tensor copied(const Tensor& x) { return plain(x).copy_(x); }
 // x itself where the kernels read it in place: contiguous columns, row strides below 2^22, for
-// bfloat16 even strides and a start on a 4-byte boundary; else a contiguous copy
-Tensor columns(const Tensor& x) {
+// bfloat16 even strides and a start on a 4-byte boundary; else a contiguous copy.  `apart`: rows
+// must not share elements either (the backward pass's queries).
+Tensor columns(const Tensor& x, bool apart = false) {
   const int64_t s0 = x.stride(0), s1 = x.stride(1);
-  bool ok = x.stride(2) == 1 && s0 >= 0 && s0 < (1 << 22) && pairs(x);
+  bool ok = x.stride(2) == 1 && s0 >= (apart ? x.size(2) : 0) && s0 < (1 << 22) && pairs(x);
   if (is16(x)) ok = ok && s0 % 2 == 0 && s1 % 2 == 0;
   return ok ? x : copied(x);
 }
@@ -159,7 +160,7 @@ Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, cons
 struct JaggedAttention : torch::autograd::Function<JaggedAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& offsets,
                         bool causal, double scale) {
-    const Tensor q = columns(q0), k = columns(k0), v = columns(v0);
+    const Tensor q = columns(q0, true), k = columns(k0), v = columns(v0);
     Tensor low, lse;
     const Tensor out = attention_forward(q, k, v, offsets, causal, scale, &low, &lse);
     ctx->save_for_backward({q, k, v, offsets, out, low, lse});

@@ -465,3 +465,23 @@ def test_contiguous_views_that_start_anywhere(dtype):
     ends = torch.tensor([0, 1], device="cuda")
     for x, y in zip(run(*one, ends, dout[:1]), run(*(t[:1].clone() for t in (q, k, v)), ends, dout[:1])):
         assert torch.equal(x, y)
+
+
+@DTYPES
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+@pytest.mark.parametrize("which", ["q", "k", "v", "all"])
+@pytest.mark.parametrize("step", [0, 24], ids=["one row for all", "overlapping"])
+def test_rows_narrower_than_their_width(step, which, causal, dtype):
+    """Rows that are one row, or that share columns with the next: the tile behind a sequence's end
+    holds real values then, with scores in the hundreds, and no part of the sums."""
+    q, k, v, offsets, dout = make([1, 33, 0, 70, 127], 2, 2, 40, 40, dtype)
+    rows = int(offsets[-1])
+
+    def narrow(t):
+        flat = (20.0 * t).to(dtype).reshape(-1)
+        return flat.as_strided((rows, 2, 40), (step, 40, 1))
+
+    q, k, v = (narrow(t) if which in (n, "all") else t for n, t in zip("qkv", (q, k, v)))
+    if which == "q":
+        k = (20.0 * k).to(dtype)
+    check(q, k, v, offsets, dout, causal=causal)

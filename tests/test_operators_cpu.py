@@ -101,3 +101,10 @@ def test_layer_norm_postprocessor_on_the_cpu_is_torchs():
     y = LayerNormEmbeddingPostprocessor(50)(x)
     assert torch.equal(y, torch.nn.functional.layer_norm(x[..., :50], (50,), eps=1e-6))
     assert torch.autograd.gradcheck(LayerNormEmbeddingPostprocessor(6), (x[0, :2, :8].detach().requires_grad_(True),))
+
+
+def test_attention_backward_refuses_queries_that_share_elements():
+    """The key rows' pass takes rows past a sequence's end as zeros, which such rows are not."""
+    for ld in (0, 4):
+        with pytest.raises(_lib.GrError, match="query rows"):
+            _lib.call("gr_jagged_attn_bwd", *attn(ld_q=ld), *[P] * 8, 1 << 20, None)
