@@ -7,7 +7,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
 #include <cstring>
@@ -157,6 +157,13 @@ Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, cons
   return out;
 }
 
+// The history of gradients made under create_graph: its edges are what they depend on (q, k, v and
+// the output's gradient), so that every way to a second derivative meets it.
+struct NoSecondDerivative : torch::autograd::Node {
+  explicit NoSecondDerivative(torch::autograd::edge_list&& edges) : Node(std::move(edges)) {}
+  variable_list apply(variable_list&&) override { TORCH_CHECK(false, "jagged_attention: no second derivative"); }
+};
+
 struct JaggedAttention : torch::autograd::Function<JaggedAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& offsets,
                         bool causal, double scale) {
@@ -189,11 +196,11 @@ struct JaggedAttention : torch::autograd::Function<JaggedAttention> {
                              stream(q)),
            "gr_jagged_attn_bwd");
     }
-    if (at::GradMode::is_enabled()) {  // create_graph: a second derivative raises where it is taken
-      const variable_list first(got.begin(), got.begin() + 3);
-      const auto node = std::make_shared<torch::autograd::DelayedError>("jagged_attention: no second derivative", 3);
-      const variable_list marked = node->apply(variable_list(first));
-      for (int i = 0; i < 3; ++i) got[i] = marked[i];
+    if (at::GradMode::is_enabled()) {  // create_graph
+      auto edges = torch::autograd::get_current_node()->next_edges();
+      edges.push_back(torch::autograd::impl::gradient_edge(grads[0]));
+      const auto node = std::make_shared<NoSecondDerivative>(std::move(edges));
+      for (int i = 0; i < 3; ++i) torch::autograd::set_history(got[i], node);
     }
     return got;
   }

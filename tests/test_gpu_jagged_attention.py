@@ -485,3 +485,25 @@ def test_rows_narrower_than_their_width(step, which, causal, dtype):
     if which == "q":
         k = (20.0 * k).to(dtype)
     check(q, k, v, offsets, dout, causal=causal)
+
+
+def test_a_second_derivative_raises_where_it_is_taken():
+    """create_graph=True: the first gradient is the same and carries a history that raises, so that no
+    term of a sum is left out in silence."""
+    from mygenerativerecommenders_amd import ops
+    q, k, v, offsets, dout = make([40, 21], 4, 2, 16, 16, torch.float32)
+    want = run(q, k, v, offsets, dout)[1:]
+    q, k, v = (t.detach().requires_grad_(True) for t in (q, k, v))
+    grads = torch.autograd.grad(ops.jagged_attention(q, k, v, offsets), (q, k, v), dout, create_graph=True)
+    for g, w in zip(grads, want):
+        assert torch.equal(g, w) and g.requires_grad
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            torch.autograd.grad(q.square().sum() + g.square().sum(), q, retain_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        (q.square().sum() + grads[2].square().sum()).backward(retain_graph=True)
+    w = dout.clone().requires_grad_(True)  # the product with a gradient's gradient: by way of dout
+    (g,) = torch.autograd.grad(ops.jagged_attention(q, k, v, offsets), q, w, create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(g.sum() + w.sum(), w)
+    (gq,) = torch.autograd.grad(q.square().sum() + 0 * grads[0].detach().sum(), q)
+    assert torch.equal(gq, 2 * q)
