@@ -4,7 +4,9 @@
 // The C-ABI library is not linked: bind() takes the addresses of its functions, so that both
 // sides use the one that is loaded.  Arguments are checked by the Python entry points.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -50,6 +52,25 @@ bool is16(const Tensor& t) { return t.scalar_type() == at::kBFloat16; }
 Tensor floats(const Tensor& like, at::IntArrayRef size) { return at::empty(size, like.options().dtype(at::kFloat)); }
 Tensor bytes(const Tensor& like, size_t n) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
 Tensor plain(const Tensor& like) { return at::empty(like.sizes(), like.options()); }
+
+// The kernels read memory and know nothing of forward-mode tangents, batched maps and traces: these raise
+// (they would go on without the operator).  Tensors of such kinds have no memory of their own or keys
+// of their own; a trace of plain tensors shows in its mode.
+bool has_tangent(const Tensor& t) {
+  return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined();
+}
+void plain_call(const char* what, std::initializer_list<const Tensor*> inputs) {
+  using c10::DispatchKey;
+  constexpr c10::DispatchKeySet wrapped{DispatchKey::Python, DispatchKey::Functionalize, DispatchKey::FuncTorchBatched,
+                                        DispatchKey::FuncTorchGradWrapper, DispatchKey::Batched};
+  for (const Tensor* t : inputs) {
+    if (!t->defined()) continue;
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(*t), what, ": no forward-mode derivative");
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->key_set().has_any(wrapped), what, ": plain tensors only, no transformed or traced ones");
+  }
+  TORCH_CHECK_NOT_IMPLEMENTED(!c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY), what,
+                              ": cannot be traced");
+}
 
 // ---------------------------------------------------------------- layer norm
 // x as (rows, D) with contiguous columns: a view wherever its strides allow
@@ -122,6 +143,7 @@ bool wanted(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
   const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  plain_call("layer_norm", {&x, &w, &b});
   if (at::GradMode::is_enabled() && (wanted(x) || wanted(w) || wanted(b))) return LayerNorm::apply(x, weight, bias, eps);
   return norm_forward(x, w, b, eps, nullptr);
 }
@@ -207,6 +229,7 @@ struct JaggedAttention : torch::autograd::Function<JaggedAttention> {
 };
 
 Tensor jagged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& offsets, bool causal, double scale) {
+  plain_call("jagged_attention", {&q, &k, &v, &offsets});
   if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v)))
     return JaggedAttention::apply(q, k, v, offsets, causal, scale);
   return attention_forward(columns(q), columns(k), columns(v), offsets, causal, scale, nullptr, nullptr);

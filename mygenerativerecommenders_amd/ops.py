@@ -202,7 +202,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     weight and bias).  x is float32 or bfloat16 with any strides (a view whose rows have
     one stride is read in place); weight and bias (D,), each optional, share one of the two
     types.  Sums are fp32; the output has x's type, the weight's and bias's gradients are
-    summed over the rows in a fixed order."""
+    summed over the rows in a fixed order.  Forward-mode derivatives and traces raise
+    NotImplementedError."""
     _lib.require_gpu(x, weight, bias)
     if x.dtype not in _FLOATS:
         raise TypeError("layer_norm: float32 or bfloat16 expected")
@@ -1236,7 +1237,8 @@ def jagged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     score is beyond 5.8e6 in magnitude (it sees masked keys alone, say) gives no gradient: its log-sum does
     not hold in fp32.  Softmax and sums are fp32; bfloat16 probabilities enter the products
     rounded to bfloat16, with their rounding errors as a second operand where a gradient is wanted
-    (so such outputs can differ in the last bit).  No atomics: the same bits every run."""
+    (so such outputs can differ in the last bit).  No atomics: the same bits every run.  Second and
+    forward-mode derivatives and traces raise."""
     _lib.require_gpu(q, k, v, offsets)
     if q.dtype not in _FLOATS or k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError("jagged_attention: q, k and v must be float32 or bfloat16, all the same")

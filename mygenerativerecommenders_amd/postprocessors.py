@@ -11,6 +11,7 @@ import abc
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.forward_ad import unpack_dual
 
 from . import ops
 
@@ -42,8 +43,8 @@ class L2NormEmbeddingPostprocessor(OutputPostprocessorModule):
 
 class LayerNormEmbeddingPostprocessor(OutputPostprocessorModule):
     """postprocessors.py:59-80.  float32 and bfloat16 rows on the GPU run ``ops.layer_norm``;
-    everything else (CPU tensors, other types, autocast, traced or transformed calls) is torch's
-    ``F.layer_norm``."""
+    everything else (CPU tensors, other types, autocast, forward-mode derivatives, traced or transformed
+    calls) is torch's ``F.layer_norm``."""
 
     def __init__(self, embedding_dim: int, eps: float = 1e-6) -> None:
         super().__init__()
@@ -57,6 +58,7 @@ class LayerNormEmbeddingPostprocessor(OutputPostprocessorModule):
         output_embeddings = output_embeddings[..., : self._embedding_dim]
         if (output_embeddings.is_cuda and output_embeddings.dtype in (torch.float32, torch.bfloat16)
                 and output_embeddings.shape[-1] == self._embedding_dim
+                and unpack_dual(output_embeddings).tangent is None
                 and not torch.is_autocast_enabled() and not torch.compiler.is_compiling()
                 and not torch._C._are_functorch_transforms_active()):
             return ops.layer_norm(output_embeddings, eps=self._eps)

@@ -507,3 +507,26 @@ def test_a_second_derivative_raises_where_it_is_taken():
         torch.autograd.grad(g.sum() + w.sum(), w)
     (gq,) = torch.autograd.grad(q.square().sum() + 0 * grads[0].detach().sum(), q)
     assert torch.equal(gq, 2 * q)
+
+
+def test_no_derivative_is_dropped_in_silence():
+    """Forward-mode derivatives and traces, which the kernels know nothing of, raise; a batched map runs
+    them in a loop, a compiled function around them."""
+    import torch.autograd.forward_ad as fw
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from mygenerativerecommenders_amd import ops
+    q, k, v, offsets, _ = make([10, 5], 4, 2, 16, 16, torch.float32)
+    for grad in (False, True):
+        with fw.dual_level():
+            for i in range(3):
+                args = [q, k, v]
+                args[i] = fw.make_dual(args[i].clone().requires_grad_(grad), torch.ones_like(args[i]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    ops.jagged_attention(*args, offsets)
+    f = lambda x: ops.jagged_attention(x, k, v, offsets)  # noqa: E731
+    with pytest.raises(NotImplementedError, match="traced"):
+        make_fx(f)(q)
+    with pytest.raises(NotImplementedError, match="plain tensors"):
+        torch.func.grad(lambda x: f(x).sum())(q)
+    assert torch.equal(torch.func.vmap(f)(torch.stack([q, 2 * q])), torch.stack([f(q), f(2 * q)]))
+    assert torch.equal(torch.compile(f, backend="eager")(q), f(q))

@@ -271,3 +271,42 @@ def test_refusals_and_empty():
     e, w2, b2 = (t.detach().requires_grad_(True) for t in (x[:0], w, b))
     ops.layer_norm(e, w2, b2).sum().backward()
     assert e.grad.shape == (0, 16) and (w2.grad == 0).all() and (b2.grad == 0).all()
+
+
+def test_no_derivative_is_dropped_in_silence():
+    """Forward-mode derivatives and traces, which the kernels know nothing of, raise; a batched map runs
+    them in a loop, a compiled function around them."""
+    import torch.autograd.forward_ad as fw
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from mygenerativerecommenders_amd import ops
+    x, w, b = inputs(6, 16, torch.float32, torch.float32)
+    for grad in (False, True):
+        with fw.dual_level():
+            for i, t in enumerate((x, w, b)):
+                args = [x, w, b]
+                args[i] = fw.make_dual(t.clone().requires_grad_(grad), torch.ones_like(t))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    ops.layer_norm(*args)
+    f = lambda t: ops.layer_norm(t, w, b)  # noqa: E731
+    with pytest.raises(NotImplementedError, match="traced"):
+        make_fx(f)(x)
+    with pytest.raises(NotImplementedError, match="plain tensors"):
+        torch.func.grad(lambda t: f(t).sum())(x)
+    assert torch.equal(torch.func.vmap(f)(torch.stack([x, 2 * x])), torch.stack([f(x), f(2 * x)]))
+    assert torch.equal(torch.compile(f, backend="eager")(x), f(x))
+
+
+def test_postprocessor_keeps_the_forward_mode_derivative():
+    import torch.autograd.forward_ad as fw
+    from mygenerativerecommenders_amd.postprocessors import LayerNormEmbeddingPostprocessor
+    x, way = torch.randn(2, 6, 16, device="cuda")
+    m = LayerNormEmbeddingPostprocessor(12)
+    norm = lambda t: torch.nn.functional.layer_norm(t[..., :12], (12,), eps=1e-6)  # noqa: E731
+    for grad in (False, True):
+        with fw.dual_level():
+            dual = fw.make_dual(x.clone().requires_grad_(grad), way)
+            got, want = (fw.unpack_dual(f(dual)).tangent for f in (m, norm))
+            assert want is not None and torch.equal(got, want)
+    leaf = x.clone().requires_grad_(True)
+    name = m(leaf).grad_fn.name()
+    assert "LayerNorm" in name and "Native" not in name

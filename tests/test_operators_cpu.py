@@ -108,3 +108,23 @@ def test_attention_backward_refuses_queries_that_share_elements():
     for ld in (0, 4):
         with pytest.raises(_lib.GrError, match="query rows"):
             _lib.call("gr_jagged_attn_bwd", *attn(ld_q=ld), *[P] * 8, 1 << 20, None)
+
+
+def test_operators_refuse_what_they_would_drop():
+    """Tangents and traces, before anything of the GPU's is asked."""
+    import torch.autograd.forward_ad as fw
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, q, offsets = torch.randn(3, 8), torch.randn(3, 2, 8), torch.tensor([0, 3])
+    norm = lambda t: _lib.nodes().layer_norm.default(t, None, None, 1e-6)  # noqa: E731
+    attend = lambda t: _lib.nodes().jagged_attention.default(t, t, t, offsets, True, 1.0)  # noqa: E731
+    for f, t in ((norm, x), (attend, q)):
+        with fw.dual_level():
+            for grad in (False, True):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    f(fw.make_dual(t.clone().requires_grad_(grad), torch.ones_like(t)))
+        with pytest.raises(NotImplementedError, match="traced"):
+            make_fx(f)(t)
+        with pytest.raises(NotImplementedError):
+            make_fx(f, tracing_mode="fake")(t)
+        with pytest.raises(NotImplementedError):
+            torch.func.jvp(f, (t,), (t,))
