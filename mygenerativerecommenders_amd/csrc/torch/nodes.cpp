@@ -6,7 +6,6 @@
 #include <ATen/ATen.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
-#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -69,9 +68,8 @@ void plain_call(const char* what, std::initializer_list<const Tensor*> inputs) {
     TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(*t), what, ": no forward-mode derivative");
     TORCH_CHECK_NOT_IMPLEMENTED(!t->key_set().has_any(wrapped), what, ": plain tensors only, no transformed or traced ones");
   }
-  TORCH_CHECK_NOT_IMPLEMENTED(!c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY) &&
-                                  !c10::impl::tls_is_dispatch_key_included(DispatchKey::PreDispatch),
-                              what, ": cannot be traced");
+  TORCH_CHECK_NOT_IMPLEMENTED(!c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY), what,
+                              ": cannot be traced");
 }
 
 // ---------------------------------------------------------------- layer norm

@@ -128,12 +128,3 @@ def test_operators_refuse_what_they_would_drop():
             make_fx(f, tracing_mode="fake")(t)
         with pytest.raises(NotImplementedError):
             torch.func.jvp(f, (t,), (t,))
-
-
-def test_operators_refuse_a_trace_before_dispatch():
-    from torch.fx.experimental.proxy_tensor import make_fx
-    x, q, offsets = torch.randn(3, 8), torch.randn(3, 2, 8), torch.tensor([0, 3])
-    for f, t in ((lambda t: _lib.nodes().layer_norm.default(t, None, None, 1e-6), x),
-                 (lambda t: _lib.nodes().jagged_attention.default(t, t, t, offsets, True, 1.0), q)):
-        with pytest.raises(NotImplementedError, match="traced"):
-            make_fx(f, pre_dispatch=True)(t)
