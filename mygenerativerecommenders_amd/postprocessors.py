@@ -56,11 +56,18 @@ class LayerNormEmbeddingPostprocessor(OutputPostprocessorModule):
 
     def forward(self, output_embeddings: torch.Tensor) -> torch.Tensor:
         output_embeddings = output_embeddings[..., : self._embedding_dim]
-        if (output_embeddings.is_cuda and output_embeddings.dtype in (torch.float32, torch.bfloat16)
-                and output_embeddings.shape[-1] == self._embedding_dim
-                and unpack_dual(output_embeddings).tangent is None
-                and not torch.is_autocast_enabled() and not torch.compiler.is_compiling()
-                and not torch._C._are_functorch_transforms_active()):
-            return ops.layer_norm(output_embeddings, eps=self._eps)
+        if not torch.jit.is_scripting():
+            if _kernel_takes(output_embeddings, self._embedding_dim):
+                return ops.layer_norm(output_embeddings, eps=self._eps)
         return F.layer_norm(output_embeddings, normalized_shape=(self._embedding_dim,),
                             eps=self._eps)
+
+
+def _kernel_takes(x, dim: int) -> bool:
+    """Whether ``ops.layer_norm`` runs x, a plain tensor that no tracer or transform watches."""
+    return (not torch.jit.is_tracing() and not torch.compiler.is_compiling()
+            and type(x) is torch.Tensor and x.is_cuda and x.dtype in (torch.float32, torch.bfloat16)
+            and 0 < dim == x.shape[-1] and unpack_dual(x).tangent is None
+            and not torch.is_autocast_enabled() and not torch._C._are_functorch_transforms_active()
+            and not torch._C._len_torch_dispatch_stack()
+            and not torch._C._dispatch_tls_is_dispatch_key_included(torch._C.DispatchKey.PreDispatch))

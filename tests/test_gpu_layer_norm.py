@@ -310,3 +310,19 @@ def test_postprocessor_keeps_the_forward_mode_derivative():
     leaf = x.clone().requires_grad_(True)
     name = m(leaf).grad_fn.name()
     assert "LayerNorm" in name and "Native" not in name
+
+
+def test_postprocessor_traces_to_torchs_norm():
+    """Every tracer sees torch's layer norm, and what it made runs without this package's operators."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from mygenerativerecommenders_amd.postprocessors import LayerNormEmbeddingPostprocessor
+    x, other = torch.randn(2, 6, 16, device="cuda")
+    m = LayerNormEmbeddingPostprocessor(12)
+    norm = lambda t: torch.nn.functional.layer_norm(t[..., :12], (12,), eps=1e-6)  # noqa: E731
+    traced = [make_fx(m)(x), make_fx(m, tracing_mode="fake")(x), make_fx(m, pre_dispatch=True)(x),
+              torch.jit.trace(m, x), torch.fx.symbolic_trace(m),
+              torch.jit.script(m), torch.export.export(m, (x,)).module(), torch.compile(m, backend="eager")]
+    for t in traced:
+        assert torch.equal(t(other), norm(other))
+    assert all("layer_norm" in t.code and "gr_amd" not in t.code for t in traced[:-1])
+    assert torch.allclose(torch.func.vmap(m)(torch.stack([x, other])), torch.stack([norm(x), norm(other)]), atol=1e-5)

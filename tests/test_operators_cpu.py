@@ -128,3 +128,12 @@ def test_operators_refuse_what_they_would_drop():
             make_fx(f, tracing_mode="fake")(t)
         with pytest.raises(NotImplementedError):
             torch.func.jvp(f, (t,), (t,))
+
+
+def test_layer_norm_postprocessor_can_be_traced_and_scripted():
+    """Symbolic proxies and TorchScript reach torch's norm as they do without a kernel."""
+    from mygenerativerecommenders_amd.postprocessors import LayerNormEmbeddingPostprocessor
+    m, x = LayerNormEmbeddingPostprocessor(5), torch.randn(4, 8)
+    want = torch.nn.functional.layer_norm(x[..., :5], (5,), eps=1e-6)
+    for t in (torch.fx.symbolic_trace(m), torch.jit.script(m), torch.jit.trace(m, x)):
+        assert torch.equal(t(x), want) and "layer_norm" in t.code
