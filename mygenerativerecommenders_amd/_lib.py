@@ -104,7 +104,9 @@ def nodes():
                 raise RuntimeError(f"{NODES_PATH} is missing: build it with `python -c 'import "
                                    "__graft_entry__ as g; g.build()'`.")
             torch.ops.load_library(NODES_PATH)
-            torch.ops.gr_amd.bind([ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in _BOUND])
+            table = (ctypes.c_void_p * len(_BOUND))(*(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in _BOUND))
+            if ctypes.CDLL(NODES_PATH).gr_torch_bind(table, len(_BOUND)) != 0:
+                raise RuntimeError(f"{NODES_PATH} does not belong to this package's version: build it again")
             _nodes = torch.ops.gr_amd
     return _nodes
 

@@ -1,8 +1,8 @@
 // Autograd nodes and the optimizer's list call over the C-ABI entries, as torch operators
 // (gr_amd::*).  A backward pass runs on one of torch's own threads: written in Python it takes
 // the interpreter there and back, some 45 us a call, more than the kernels of a small batch.
-// The C-ABI library is not linked: bind() takes the addresses of its functions, so that both
-// sides use the one that is loaded.  Arguments are checked by the Python entry points.
+// The C-ABI library is not linked: gr_torch_bind() takes the addresses of its functions, so that both
+// sides use the one that is loaded (no operator, or a trace that makes the first call would hold them).  Arguments are checked by the Python entry points.
 #include <ATen/ATen.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
@@ -36,12 +36,7 @@ struct Entries {
 };
 Entries e{};
 
-void bind(at::IntArrayRef addresses) {
-  TORCH_CHECK(addresses.size() * sizeof(void*) == sizeof(Entries), "gr_amd::bind: ", addresses.size(), " addresses");
-  static_assert(sizeof(int64_t) == sizeof(void*));
-  std::memcpy(&e, addresses.data(), sizeof(Entries));
-}
-
+void bound() { TORCH_CHECK(e.last_error, "gr_amd: import mygenerativerecommenders_amd and call _lib.nodes() first"); }
 void done(int status, const char* what) {
   TORCH_CHECK(status == 0, what, " failed (status ", status, "): ", e.last_error());
 }
@@ -60,6 +55,7 @@ bool has_tangent(const Tensor& t) {
   return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined();
 }
 void plain_call(const char* what, std::initializer_list<const Tensor*> inputs) {
+  bound();
   using c10::DispatchKey;
   constexpr c10::DispatchKeySet wrapped{DispatchKey::Python, DispatchKey::Functionalize, DispatchKey::FuncTorchBatched,
                                         DispatchKey::FuncTorchGradWrapper, DispatchKey::Batched};
@@ -241,6 +237,7 @@ Tensor jagged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
 void adamw8_step(at::TensorList params, const Tensor& exp_avg, const Tensor& exp_avg_scale, const Tensor& exp_avg_sq,
                  const Tensor& exp_avg_sq_scale, const Tensor& step, const Tensor& counters, double lr, double beta1,
                  double beta2, double eps, double weight_decay) {
+  bound();
   const size_t n = params.size();
   std::vector<float*> p(n);
   std::vector<const float*> g(n);
@@ -270,7 +267,6 @@ void adamw8_step(at::TensorList params, const Tensor& exp_avg, const Tensor& exp
 }  // namespace
 
 TORCH_LIBRARY(gr_amd, m) {
-  m.def("bind(int[] addresses) -> ()", bind);
   m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor", layer_norm);
   m.def("jagged_attention(Tensor q, Tensor k, Tensor v, Tensor offsets, bool causal, float scale) -> Tensor",
         jagged_attention);
@@ -278,4 +274,10 @@ TORCH_LIBRARY(gr_amd, m) {
       "adamw8_step(Tensor[] params, Tensor exp_avg, Tensor exp_avg_scale, Tensor exp_avg_sq, Tensor exp_avg_sq_scale, "
       "Tensor step, Tensor counters, float lr, float beta1, float beta2, float eps, float weight_decay) -> ()",
       adamw8_step);
+}
+
+extern "C" __attribute__((visibility("default"))) int gr_torch_bind(const void* const* addresses, int n) {
+  if (n * sizeof(void*) != sizeof(Entries)) return 1;
+  std::memcpy(&e, addresses, sizeof(Entries));
+  return 0;
 }

@@ -137,3 +137,25 @@ def test_layer_norm_postprocessor_can_be_traced_and_scripted():
     want = torch.nn.functional.layer_norm(x[..., :5], (5,), eps=1e-6)
     for t in (torch.fx.symbolic_trace(m), torch.jit.script(m), torch.jit.trace(m, x)):
         assert torch.equal(t(x), want) and "layer_norm" in t.code
+
+
+def test_a_trace_that_makes_the_first_call_holds_no_addresses():
+    """In a process of its own, as a process loads the operators once."""
+    import subprocess
+    import sys
+    code = ("import torch; from torch.fx.experimental.proxy_tensor import make_fx\n"
+            "from mygenerativerecommenders_amd import _lib\n"
+            "g = make_fx(lambda x: (_lib.nodes(), x + 1)[1], pre_dispatch=True)(torch.zeros(3))\n"
+            "assert 'gr_amd' not in g.code, g.code\n")
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=120)
+
+
+def test_the_operators_alone_raise():
+    """A process that loads libgr_torch.so by itself (for a saved trace, say) has no kernels behind it."""
+    import subprocess
+    import sys
+    code = (f"import torch; torch.ops.load_library({_lib.NODES_PATH!r})\n"
+            "try:\n    torch.ops.gr_amd.layer_norm(torch.zeros(2, 8), None, None, 1e-6)\n"
+            "except RuntimeError as e:\n    assert '_lib.nodes()' in str(e), e\n"
+            "else:\n    raise SystemExit(1)\n")
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=120)
