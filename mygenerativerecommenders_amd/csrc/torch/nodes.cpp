@@ -69,11 +69,13 @@ void plain_call(const char* what, std::initializer_list<const Tensor*> inputs) {
 }
 
 // ---------------------------------------------------------------- layer norm
-// x as (rows, D) with contiguous columns: a view wherever its strides allow
+// x as (rows, D) with contiguous columns and rows that are D apart, or one: a view wherever its
+// strides allow
 Tensor rows_of(const Tensor& x) {
   const int64_t d = x.size(-1);
   const Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, d});
-  return d == 1 || x2.stride(1) == 1 ? x2 : x2.contiguous();
+  const bool apart = x2.size(0) <= 1 || x2.stride(0) == 0 || x2.stride(0) >= d;
+  return (d == 1 || x2.stride(1) == 1) && apart ? x2 : x2.contiguous();
 }
 
 int norm_types(const Tensor& x, const Tensor& weight, const Tensor& bias) {

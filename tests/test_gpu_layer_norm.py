@@ -326,3 +326,19 @@ def test_postprocessor_traces_to_torchs_norm():
         assert torch.equal(t(other), norm(other))
     assert all("layer_norm" in t.code and "gr_amd" not in t.code for t in traced[:-1])
     assert torch.allclose(torch.func.vmap(m)(torch.stack([x, other])), torch.stack([norm(x), norm(other)]), atol=1e-5)
+
+
+@DTYPES
+def test_overlapping_rows(dtype):
+    """Rows that share columns with the next (a window moved by less than a row)."""
+    from mygenerativerecommenders_amd.postprocessors import LayerNormEmbeddingPostprocessor
+    g = torch.Generator(device="cuda").manual_seed(3)
+    line = torch.randn(400, device="cuda", generator=g).to(dtype)
+    _, w, b = inputs(2, 50, dtype, torch.float32)
+    for step in (1, 7, 49):
+        x = line.unfold(0, 50, step)
+        assert x.stride() == (step, 1)
+        check(x, w, b)
+        y = LayerNormEmbeddingPostprocessor(50)(x)
+        (ref, lim), *_ = reference(x, None, None, 1e-6, torch.zeros_like(x))
+        assert ((y.double() - ref).abs() <= lim + 1e-30).all()
