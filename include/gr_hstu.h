@@ -295,7 +295,7 @@ GR_API int gr_adamw8_step(float* const* params, const float* const* grads, const
                           double eps, double weight_decay, void* stream);
 
 /* ---------------------------------------------------------------- layer norm (ABI 19)
- * Rows of D elements, row strides ld_* in elements (>= D, or 0 for one row read for all),
+ * Rows of D < 2^29 elements, row strides ld_* in elements (>= D, or 0 for one row read for all),
  * no alignment beyond the element's.  types: bit 0: x, y, dy, dx are bf16 (else fp32);
  * bit 1: weight, bias and their gradients are bf16 (else fp32).  weight / bias may be NULL.
  * Forward: y = (x - mu) r weight + bias with mu, r = 1 / sqrt(var + eps) of each row (var

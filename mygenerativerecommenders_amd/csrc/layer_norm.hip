@@ -21,6 +21,8 @@
 
 namespace gr {
 
+constexpr int LN_COLUMNS = 1 << 29;  // rows are narrower: columns are counted in 32 bits, up to 2 D and a step
+
 struct LnArgs {
   const void* x;
   int64_t ld_x;
@@ -477,7 +479,7 @@ extern "C" {
 
 int gr_layer_norm_fwd(const void* x, int64_t ld_x, int64_t rows, int D, const void* weight, const void* bias,
                       int types, float eps, void* y, int64_t ld_y, float* stats, void* stream) {
-  GR_REQUIRE(rows >= 0 && D >= 1 && types >= 0 && types < 4 && (rows == 0 || (x && y)), "gr_layer_norm_fwd: bad args");
+  GR_REQUIRE(rows >= 0 && D >= 1 && D < gr::LN_COLUMNS && types >= 0 && types < 4 && (rows == 0 || (x && y)), "gr_layer_norm_fwd: bad args");
   GR_REQUIRE(rows <= 1 || ((ld_x >= D || ld_x == 0) && ld_y >= D), "gr_layer_norm_fwd: row strides below D");
   if (rows == 0) return 0;
   const hipStream_t st = (hipStream_t)stream;
@@ -513,7 +515,7 @@ size_t gr_layer_norm_bwd_workspace_size(int64_t rows, int D, int types) {
 int gr_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int64_t rows, int D,
                       const void* weight, int types, const float* stats, void* dx, int64_t ld_dx, void* dweight,
                       void* dbias, void* workspace, size_t ws_bytes, void* stream) {
-  GR_REQUIRE(rows >= 0 && D >= 1 && types >= 0 && types < 4 && (rows == 0 || (dy && x && stats)),
+  GR_REQUIRE(rows >= 0 && D >= 1 && D < gr::LN_COLUMNS && types >= 0 && types < 4 && (rows == 0 || (dy && x && stats)),
              "gr_layer_norm_bwd: bad args");
   GR_REQUIRE(rows <= 1 || ((ld_x >= D || ld_x == 0) && (ld_dy >= D || ld_dy == 0) && (!dx || ld_dx >= D)),
              "gr_layer_norm_bwd: row strides below D");

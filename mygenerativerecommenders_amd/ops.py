@@ -193,6 +193,7 @@ def l2_normalize(x: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
 # ------------------------------------------------------------------ layer norm
 
 _FLOATS = (torch.float32, torch.bfloat16)
+LN_COLUMNS = 1 << 29  # the kernels' rows are narrower
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -207,8 +208,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     _lib.require_gpu(x, weight, bias)
     if x.dtype not in _FLOATS:
         raise TypeError("layer_norm: float32 or bfloat16 expected")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("layer_norm: a last dimension of at least one element expected")
+    if x.dim() < 1 or not 1 <= x.shape[-1] < LN_COLUMNS:
+        raise ValueError("layer_norm: a last dimension of 1 to 2^29 - 1 elements expected")
     params = [t for t in (weight, bias) if t is not None]
     for t in params:
         if t.dtype not in _FLOATS or t.dtype != params[0].dtype:

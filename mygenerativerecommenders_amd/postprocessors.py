@@ -67,7 +67,7 @@ def _kernel_takes(x, dim: int) -> bool:
     """Whether ``ops.layer_norm`` runs x, a plain tensor that no tracer or transform watches."""
     return (not torch.jit.is_tracing() and not torch.compiler.is_compiling()
             and type(x) is torch.Tensor and x.is_cuda and x.dtype in (torch.float32, torch.bfloat16)
-            and 0 < dim == x.shape[-1] and unpack_dual(x).tangent is None
+            and 0 < dim == x.shape[-1] < ops.LN_COLUMNS and unpack_dual(x).tangent is None
             and not torch.is_autocast_enabled() and not torch._C._are_functorch_transforms_active()
             and not torch._C._len_torch_dispatch_stack()
             and not torch._C._dispatch_tls_is_dispatch_key_included(torch._C.DispatchKey.PreDispatch))

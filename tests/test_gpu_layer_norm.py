@@ -342,3 +342,11 @@ def test_overlapping_rows(dtype):
         y = LayerNormEmbeddingPostprocessor(50)(x)
         (ref, lim), *_ = reference(x, None, None, 1e-6, torch.zeros_like(x))
         assert ((y.double() - ref).abs() <= lim + 1e-30).all()
+
+
+def test_refuses_rows_that_32_bits_do_not_count():
+    """A width of 2^32 + 50 is not one of 50; the rows are one element, expanded."""
+    from mygenerativerecommenders_amd import ops
+    for d in (1 << 29, (1 << 32) + 50):
+        with pytest.raises(ValueError, match="2\\^29"):
+            ops.layer_norm(torch.zeros(1, 1, device="cuda").expand(2, d))

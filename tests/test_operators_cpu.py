@@ -159,3 +159,11 @@ def test_the_operators_alone_raise():
             "except RuntimeError as e:\n    assert '_lib.nodes()' in str(e), e\n"
             "else:\n    raise SystemExit(1)\n")
     subprocess.run([sys.executable, "-c", code], check=True, timeout=120)
+
+
+@pytest.mark.parametrize("D", [1 << 29, (1 << 31) - 1])
+def test_layer_norm_refuses_rows_that_32_bits_do_not_count(D):
+    with pytest.raises(_lib.GrError, match="gr_layer_norm_fwd"):
+        _lib.call("gr_layer_norm_fwd", P, D, 1, D, None, None, 0, 1e-6, P, D, None, None)
+    with pytest.raises(_lib.GrError, match="gr_layer_norm_bwd: bad args"):
+        _lib.call("gr_layer_norm_bwd", P, D, P, D, 1, D, None, 0, P, P, D, None, None, None, 0, None)
