@@ -1253,8 +1253,10 @@ def jagged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         raise ValueError(f"jagged_attention: {H} query heads are no multiple of {k.shape[1]} key heads")
     if not (1 <= d <= 256 and 1 <= v.shape[2] <= 256):
         raise ValueError(f"jagged_attention: head widths {d}, {v.shape[2]} outside [1, 256]")
-    if offsets.dim() != 1 or offsets.numel() < 1 or offsets.is_floating_point() or offsets.dtype == torch.bool:
+    if offsets.dim() != 1 or offsets.is_floating_point() or offsets.dtype == torch.bool:
         raise ValueError("jagged_attention: offsets must be (B + 1,) integers")
+    if not 1 <= offsets.numel() < 1 << 31:  # counted in 32 bits
+        raise ValueError(f"jagged_attention: {offsets.numel()} offsets, expected 1 to 2^31 - 1")
     if any(t.device != q.device for t in (k, v, offsets)):
         raise ValueError("jagged_attention: all tensors must be on one device")
     scale = d ** -0.5 if scale is None else float(scale)

@@ -530,3 +530,12 @@ def test_no_derivative_is_dropped_in_silence():
         torch.func.grad(lambda x: f(x).sum())(q)
     assert torch.equal(torch.func.vmap(f)(torch.stack([q, 2 * q])), torch.stack([f(q), f(2 * q)]))
     assert torch.equal(torch.compile(f, backend="eager")(q), f(q))
+
+
+def test_refuses_offsets_that_32_bits_do_not_count():
+    """2^32 + 2 offsets (one element, expanded) are not two."""
+    from mygenerativerecommenders_amd import ops
+    q, k, v, offsets, _ = make([10, 5], 4, 2, 16, 16, torch.float32)
+    for n in (1 << 31, (1 << 32) + 2):
+        with pytest.raises(ValueError, match="offsets"):
+            ops.jagged_attention(q, k, v, offsets[:1].expand(n))
