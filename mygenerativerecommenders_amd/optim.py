@@ -48,28 +48,28 @@ class FlatAdamW(torch.optim.Optimizer):
         if fs is not None:
             return fs
         params = group["params"]
-        dev = params[0].device
-        for p in params:
-            if p.device != dev or p.dtype != torch.float32 or not p.is_contiguous() or not p.is_cuda:
-                raise TypeError("FlatAdamW: contiguous fp32 CUDA parameters on one device expected")
-        if self._bits == 8:
-            return self._group_state8(gi, params, dev)
+        if not self._takes(params):
+            raise TypeError("FlatAdamW: contiguous fp32 CUDA parameters on one device expected")
+        fs = self._buffers8(params) if self._bits == 8 else self._buffers32(params)
+        self._fill(fs, params)
+        self._flat[gi] = fs
+        return fs
+
+    def _takes(self, params: list) -> bool:
+        return all(p.device == params[0].device and p.dtype == torch.float32 and p.is_contiguous() and p.is_cuda
+                   for p in params)
+
+    def _buffers32(self, params: list) -> dict:
         offs = np.zeros(len(params), np.int64)
         o = 0
         for i, p in enumerate(params):
             offs[i] = o
             o += (p.numel() + 3) // 4 * 4  # 16-byte aligned moments (float4 path)
-        m = torch.zeros(o, dtype=torch.float32, device=dev)
-        v = torch.zeros(o, dtype=torch.float32, device=dev)
-        step = torch.zeros(1, dtype=torch.float32, device=dev)
-        done = torch.zeros(1, dtype=torch.int32, device=dev)
-        for p, off in zip(params, offs.tolist()):
-            self.state[p] = {"step": step, "exp_avg": m[off:off + p.numel()].view_as(p),
-                             "exp_avg_sq": v[off:off + p.numel()].view_as(p)}
-        fs = self._flat[gi] = {"m": m, "v": v, "step": step, "done": done, "offs": offs}
-        return fs
+        new = {"dtype": torch.float32, "device": params[0].device}
+        return {"m": torch.zeros(o, **new), "v": torch.zeros(o, **new), "step": torch.zeros(1, **new),
+                "done": torch.zeros(1, dtype=torch.int32, device=params[0].device), "offs": offs}
 
-    def _group_state8(self, gi: int, params: list, dev) -> dict:
+    def _buffers8(self, params: list) -> dict:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("FlatAdamW: take a step (or load a state) before capturing one, or the "
                                "captured graph would clear the moments on every replay")
@@ -78,21 +78,40 @@ class FlatAdamW(torch.optim.Optimizer):
         for i, p in enumerate(params):
             offs[i] = o
             o += -(-p.numel() // _BLOCK) * _BLOCK  # scales belong to one tensor each
-        fs = {"exp_avg": torch.zeros(o, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn),
-              "exp_avg_scale": torch.zeros(o // _BLOCK, dtype=torch.float32, device=dev),
-              "exp_avg_sq": torch.zeros(o, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn),
-              "exp_avg_sq_scale": torch.zeros(o // _BLOCK, dtype=torch.float32, device=dev),
-              "step": torch.zeros(1, dtype=torch.float32, device=dev)}
-        for p, off in zip(params, offs.tolist()):
-            n = p.numel()
+        dev = params[0].device
+        return {"exp_avg": torch.zeros(o, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn),
+                "exp_avg_scale": torch.zeros(o // _BLOCK, dtype=torch.float32, device=dev),
+                "exp_avg_sq": torch.zeros(o, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn),
+                "exp_avg_sq_scale": torch.zeros(o // _BLOCK, dtype=torch.float32, device=dev),
+                "step": torch.zeros(1, dtype=torch.float32, device=dev),
+                "done": torch.zeros(1040, dtype=torch.int32, device=dev),  # 65 counters, 64 bytes apart
+                "offs": offs}
+
+    def _names(self) -> tuple:
+        return ("exp_avg", "exp_avg_sq") + (("exp_avg_scale", "exp_avg_sq_scale") if self._bits == 8 else ())
+
+    def _views(self, fs: dict, p, off: int) -> dict:
+        """The per-parameter state of p, whose moments start at element ``off`` of the buffers."""
+        n = p.numel()
+        if self._bits == 8:
             blocks = slice(off // _BLOCK, (off + n + _BLOCK - 1) // _BLOCK)
-            self.state[p] = {"step": fs["step"], "exp_avg": fs["exp_avg"][off:off + n].view_as(p),
-                             "exp_avg_scale": fs["exp_avg_scale"][blocks],
-                             "exp_avg_sq": fs["exp_avg_sq"][off:off + n].view_as(p),
-                             "exp_avg_sq_scale": fs["exp_avg_sq_scale"][blocks]}
-        fs["done"] = torch.zeros(1040, dtype=torch.int32, device=dev)  # 65 counters, 64 bytes apart
-        self._flat[gi] = fs
-        return fs
+            return {"step": fs["step"], "exp_avg": fs["exp_avg"][off:off + n].view_as(p),
+                    "exp_avg_scale": fs["exp_avg_scale"][blocks],
+                    "exp_avg_sq": fs["exp_avg_sq"][off:off + n].view_as(p),
+                    "exp_avg_sq_scale": fs["exp_avg_sq_scale"][blocks]}
+        return {"step": fs["step"], "exp_avg": fs["m"][off:off + n].view_as(p),
+                "exp_avg_sq": fs["v"][off:off + n].view_as(p)}
+
+    @torch.no_grad()
+    def _fill(self, fs: dict, params: list) -> None:
+        """Moves what ``self.state`` holds for the parameters (a loaded state, checked) into a group's
+        buffers, zeros where they hold nothing yet, and makes the state views of them."""
+        for p, off in zip(params, fs["offs"].tolist()):
+            loaded, self.state[p] = self.state.get(p), self._views(fs, p, off)
+            if loaded:
+                for n in self._names():
+                    self.state[p][n].copy_(loaded[n])
+                fs["step"].copy_(torch.as_tensor(loaded["step"], dtype=torch.float32).reshape(1))
 
     def flat_state(self, group: int = 0) -> dict:
         """The flat buffers behind a parameter group's per-parameter state, by torch's names
@@ -101,36 +120,61 @@ class FlatAdamW(torch.optim.Optimizer):
         64 (8 bits), in the order of the group's parameters."""
         fs = self._group_state(group, self.param_groups[group])
         if self._bits == 8:
-            return {n: t for n, t in fs.items() if n != "done"}
+            return {n: t for n, t in fs.items() if n not in ("done", "offs")}
         return {"exp_avg": fs["m"], "exp_avg_sq": fs["v"], "step": fs["step"]}
 
     def load_state_dict(self, state_dict: dict) -> None:
         """torch's, with the loaded moments copied into the flat buffers that the step reads.
-        A state of the other ``state_bits`` raises ValueError, and so do parameters of one
-        group that have taken different numbers of steps (the group has one counter)."""
-        names = ("exp_avg", "exp_avg_sq") + (("exp_avg_scale", "exp_avg_sq_scale") if self._bits == 8 else ())
-        for st in state_dict["state"].values():
-            if any(n not in st for n in names) or ("exp_avg_scale" in st) != (self._bits == 8):
-                raise ValueError(f"FlatAdamW: the loaded state does not hold {self._bits}-bit moments")
-        super().load_state_dict(state_dict)
-        loaded = {p: self.state[p] for g in self.param_groups for p in g["params"] if self.state.get(p)}
-        self._flat.clear()
-        for gi, group in enumerate(self.param_groups):
-            have = [p for p in group["params"] if p in loaded]
-            if not have:
-                continue
-            steps = {float(loaded[p]["step"]) for p in have}
-            if len(steps) > 1:
-                raise ValueError(f"FlatAdamW: parameters of one group have taken {sorted(steps)} steps")
-            with torch.no_grad():
-                self._group_state(gi, group)["step"].fill_(steps.pop())
-                for p in have:
-                    for n in names:
-                        to, x = self.state[p][n], loaded[p][n]
-                        if to.shape != x.shape:
-                            raise ValueError(f"FlatAdamW: loaded {n} has shape {tuple(x.shape)}, "
-                                             f"expected {tuple(to.shape)}")
-                        to.copy_(x)
+        A state of the other
+        ``state_bits`` raises ValueError, and so do parameters of one group that have taken
+        different numbers of steps (the group has one counter); the optimizer is then as it was."""
+        kept, fresh = (self.state, self.param_groups), {}
+        try:
+            super().load_state_dict(state_dict)
+            self._check_loaded()
+            for gi, group in enumerate(self.param_groups):
+                params = group["params"]
+                if any(self.state.get(p) for p in params):
+                    if not self._takes(params):
+                        raise TypeError("FlatAdamW: contiguous fp32 CUDA parameters on one device expected")
+                    fresh[gi] = self._buffers8(params) if self._bits == 8 else self._buffers32(params)
+                    self._fill(fresh[gi], params)
+        except BaseException:
+            self.state, self.param_groups = kept
+            raise
+        self._flat = fresh
+
+    def _check_loaded(self) -> None:
+        """Raises ValueError unless ``self.state``, as torch has loaded it, fits."""
+        names, groups, steps, there = self._names(), [], {}, []
+        for group in self.param_groups:
+            groups.append([])
+            for p in group["params"]:
+                st = self.state.get(p)
+                if not st:
+                    continue
+                if any(n not in st for n in (*names, "step")) or ("exp_avg_scale" in st) != (self._bits == 8):
+                    raise ValueError(f"FlatAdamW: the loaded state does not hold {self._bits}-bit moments")
+                for n in names:
+                    want = (-(-p.numel() // _BLOCK),) if n.endswith("scale") else tuple(p.shape)
+                    if tuple(st[n].shape) != want:
+                        raise ValueError(f"FlatAdamW: loaded {n} has shape {tuple(st[n].shape)}, expected {want}")
+                step = st["step"]
+                groups[-1].append(step)
+                if torch.is_tensor(step) and step.numel() != 1:
+                    raise ValueError(f"FlatAdamW: loaded step has shape {tuple(step.shape)}")
+                if id(step) not in steps:
+                    steps[id(step)] = step
+                    if torch.is_tensor(step) and step.is_cuda:
+                        there.append(step)
+        if there:  # one copy to the host for all
+            dev = there[0].device
+            values = torch.stack([t.detach().reshape(()).to(dev, torch.float32) for t in there]).tolist()
+            steps.update((id(t), v) for t, v in zip(there, values))
+        for group in groups:
+            taken = {float(steps[id(step)]) for step in group}
+            if len(taken) > 1:
+                raise ValueError(f"FlatAdamW: parameters of one group have taken {sorted(taken)} steps")
 
     @torch.no_grad()
     def step(self, closure=None):

@@ -319,3 +319,84 @@ def test_refusals():
     sd["state"][0] = dict(sd["state"][0], exp_avg_scale=torch.ones(2, device="cuda"))
     with pytest.raises(ValueError, match="shape"):
         FlatAdamW([p], state_bits=8).load_state_dict(sd)
+
+def pair(bits, seed=0):
+    """An optimizer after three steps, its saved state, and parameters for another."""
+    from mygenerativerecommenders_amd.optim import FlatAdamW
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    params = [torch.nn.Parameter(torch.randn(s, device="cuda", generator=g)) for s in [(50, 20), (129,), (7, 3)]]
+    opt = FlatAdamW(params, state_bits=bits, **HYPER)
+    for t in range(3):
+        gradients(params, g, t)
+        opt.step()
+    return params, opt, g
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("fault", ["steps", "shape", "missing", "scale", "groups"])
+def test_a_refused_load_changes_nothing(fault, bits):
+    """Neither the state nor the groups' values: the next step's bits are those of an optimizer that was
+    never asked."""
+    import copy
+    params, opt, g = pair(bits)
+    twins, twin, _ = pair(bits)
+    bad = copy.deepcopy(opt.state_dict())
+    bad["param_groups"][0]["lr"] = 0.5
+    st = dict(bad["state"][1])
+    if fault == "steps":
+        st["step"] = st["step"] + 1
+    elif fault == "shape":
+        st["exp_avg_sq"] = st["exp_avg_sq"][:-1]
+    elif fault == "missing":
+        del st["exp_avg"]
+    elif fault == "scale":
+        if bits == 8:
+            st["exp_avg_scale"] = st["exp_avg_scale"][:-1]
+        else:
+            st["exp_avg_scale"] = torch.ones(3, device="cuda")
+    else:
+        bad["param_groups"][0]["params"] = [0, 1]
+    bad["state"][1] = st
+    with pytest.raises(ValueError):
+        opt.load_state_dict(bad)
+    gradients(params, g, 4)
+    for p, q in zip(params, twins):
+        q.grad = p.grad.clone()
+    opt.step()
+    twin.step()
+    assert opt.param_groups[0]["lr"] == HYPER["lr"]
+    for p, q in zip(params, twins):
+        assert torch.equal(p, q)
+        assert all(same(opt.state[p][n], twin.state[q][n]) for n in opt.state[p])
+
+
+def test_a_load_reads_the_device_once():
+    """One wait for the group's step counters, however many parameters."""
+    import copy
+    import warnings
+    params, opt, g = make([(64,)] * 40, **HYPER)
+    gradients(params, g, 0)
+    opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    for st in saved["state"].values():
+        st["step"] = st["step"].clone()
+    torch.cuda.set_sync_debug_mode("warn")
+    try:
+        with warnings.catch_warnings(record=True) as seen:
+            warnings.simplefilter("always")
+            opt.load_state_dict(saved)
+            n = sum("synchronizing" in str(w.message) for w in seen)
+            float(saved["state"][0]["step"])
+            assert sum("synchronizing" in str(w.message) for w in seen) == n + 1  # they are counted
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert n <= 1
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_loads_its_own_state(bits):
+    """A state_dict's tensors are the buffers themselves."""
+    params, opt, g = pair(bits)
+    before = {n: t.clone() for n, t in opt.flat_state().items()}
+    opt.load_state_dict(opt.state_dict())
+    assert all(same(t, before[n]) for n, t in opt.flat_state().items())
