@@ -124,8 +124,8 @@ class FlatAdamW(torch.optim.Optimizer):
         return {"exp_avg": fs["m"], "exp_avg_sq": fs["v"], "step": fs["step"]}
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """torch's, with the loaded moments copied into the flat buffers that the step reads.
-        A state of the other
+        """torch's, with the loaded moments copied into the flat buffers that the step reads: those
+        that are there, so that a captured step goes on from them.  A state of the other
         ``state_bits`` raises ValueError, and so do parameters of one group that have taken
         different numbers of steps (the group has one counter); the optimizer is then as it was."""
         kept, fresh = (self.state, self.param_groups), {}
@@ -134,7 +134,7 @@ class FlatAdamW(torch.optim.Optimizer):
             self._check_loaded()
             for gi, group in enumerate(self.param_groups):
                 params = group["params"]
-                if any(self.state.get(p) for p in params):
+                if gi in self._flat or any(self.state.get(p) for p in params):
                     if not self._takes(params):
                         raise TypeError("FlatAdamW: contiguous fp32 CUDA parameters on one device expected")
                     fresh[gi] = self._buffers8(params) if self._bits == 8 else self._buffers32(params)
@@ -142,7 +142,20 @@ class FlatAdamW(torch.optim.Optimizer):
         except BaseException:
             self.state, self.param_groups = kept
             raise
-        self._flat = fresh
+        for gi in [i for i in self._flat if i not in fresh]:
+            del self._flat[gi]
+        for gi, new in fresh.items():
+            old = self._flat.setdefault(gi, new)
+            if old is new:
+                continue
+            if old["step"].device != new["step"].device or not np.array_equal(old["offs"], new["offs"]):
+                self._flat[gi] = new
+                continue
+            for n in old:  # the loaded tensors may be views of these: through the fresh ones
+                if n not in ("done", "offs"):
+                    old[n].copy_(new[n])
+            for p, off in zip(self.param_groups[gi]["params"], old["offs"].tolist()):
+                self.state[p] = self._views(old, p, off)
 
     def _check_loaded(self) -> None:
         """Raises ValueError unless ``self.state``, as torch has loaded it, fits."""

@@ -400,3 +400,49 @@ def test_loads_its_own_state(bits):
     before = {n: t.clone() for n, t in opt.flat_state().items()}
     opt.load_state_dict(opt.state_dict())
     assert all(same(t, before[n]) for n, t in opt.flat_state().items())
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_load_fills_the_buffers_of_a_captured_step(bits):
+    """The step that was captured before goes on from the loaded moments."""
+    import copy
+    params, opt, g = pair(bits)
+    saved = copy.deepcopy(opt.state_dict())
+    start = [p.detach().clone() for p in params]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    twins, twin, _ = pair(bits)
+    for t in range(3):  # away from the saved state
+        graph.replay()
+    flat = opt.flat_state()
+    opt.load_state_dict(saved)
+    assert all(a.data_ptr() == b.data_ptr() for a, b in zip(flat.values(), opt.flat_state().values()))
+    for p, s in zip(params, start):
+        p.data.copy_(s)
+    for t in range(3):
+        for p, q in zip(params, twins):
+            q.grad = torch.randn(p.shape, device="cuda", generator=g)
+            p.grad.copy_(q.grad)
+        graph.replay()
+        twin.step()
+        for p, q in zip(params, twins):
+            assert torch.equal(p, q), t
+            assert all(same(opt.state[p][n], twin.state[q][n]) for n in opt.state[p])
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_state_without_some_parameters(bits):
+    """Parameters that had no state when it was saved start from zero moments, whatever they held."""
+    import copy
+    params, opt, g = pair(bits)
+    saved = copy.deepcopy(opt.state_dict())
+    del saved["state"][1]
+    gradients(params, g, 4)
+    opt.step()
+    opt.load_state_dict(saved)
+    st = opt.state[params[1]]
+    assert all((st[n].float() == 0).all() for n in st if n != "step") and float(st["step"]) == 3
+    assert same(opt.state[params[0]]["exp_avg"], saved["state"][0]["exp_avg"])
+    opt.load_state_dict({"state": {}, "param_groups": saved["param_groups"]})
+    assert all((t.float() == 0).all() for t in opt.flat_state().values())
