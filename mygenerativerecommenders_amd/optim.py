@@ -127,18 +127,21 @@ class FlatAdamW(torch.optim.Optimizer):
         """torch's, with the loaded moments copied into the flat buffers that the step reads: those
         that are there, so that a captured step goes on from them.  A state of the other
         ``state_bits`` raises ValueError, and so do parameters of one group that have taken
-        different numbers of steps (the group has one counter); the optimizer is then as it was."""
+        different numbers of steps (the group has one counter); the optimizer is then as it was.
+        With parameters on the CPU the state waits for the first step on the GPU."""
         kept, fresh = (self.state, self.param_groups), {}
         try:
             super().load_state_dict(state_dict)
             self._check_loaded()
             for gi, group in enumerate(self.param_groups):
                 params = group["params"]
-                if gi in self._flat or any(self.state.get(p) for p in params):
-                    if not self._takes(params):
-                        raise TypeError("FlatAdamW: contiguous fp32 CUDA parameters on one device expected")
+                if params and self._takes(params) and (gi in self._flat or any(self.state.get(p) for p in params)):
                     fresh[gi] = self._buffers8(params) if self._bits == 8 else self._buffers32(params)
                     self._fill(fresh[gi], params)
+                else:  # waits, on its own: what was loaded may be another optimizer's buffers
+                    for p in params:
+                        if self.state.get(p):
+                            self.state[p] = {n: t.clone() if torch.is_tensor(t) else t for n, t in self.state[p].items()}
         except BaseException:
             self.state, self.param_groups = kept
             raise

@@ -446,3 +446,22 @@ def test_a_state_without_some_parameters(bits):
     assert same(opt.state[params[0]]["exp_avg"], saved["state"][0]["exp_avg"])
     opt.load_state_dict({"state": {}, "param_groups": saved["param_groups"]})
     assert all((t.float() == 0).all() for t in opt.flat_state().values())
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_loaded_before_the_parameters_move_to_the_gpu(bits):
+    from mygenerativerecommenders_amd.optim import FlatAdamW
+    params, opt, g = pair(bits)
+    model = torch.nn.ParameterList([torch.nn.Parameter(p.detach().cpu()) for p in params])
+    late = FlatAdamW(model.parameters(), state_bits=bits, **HYPER)
+    late.load_state_dict(opt.state_dict())
+    model.cuda()
+    gradients(params, g, 4)
+    twins = list(model.parameters())
+    for p, q in zip(params, twins):
+        q.grad = p.grad.clone()
+    opt.step()
+    late.step()
+    for p, q in zip(params, twins):
+        assert torch.equal(p, q)
+        assert all(same(opt.state[p][n], late.state[q][n]) for n in opt.state[p])
