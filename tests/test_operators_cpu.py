@@ -167,3 +167,22 @@ def test_layer_norm_refuses_rows_that_32_bits_do_not_count(D):
         _lib.call("gr_layer_norm_fwd", P, D, 1, D, None, None, 0, 1e-6, P, D, None, None)
     with pytest.raises(_lib.GrError, match="gr_layer_norm_bwd: bad args"):
         _lib.call("gr_layer_norm_bwd", P, D, P, D, 1, D, None, 0, P, P, D, None, None, None, 0, None)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_optimizer_state_loaded_on_the_cpu(bits):
+    """It waits there as it was saved, a copy of its own, and a refused one leaves it."""
+    def moments(p, step):
+        st = {"step": torch.tensor(float(step)), "exp_avg": torch.ones_like(p), "exp_avg_sq": torch.ones_like(p)}
+        blocks = -(-p.numel() // 64)
+        return dict(st, exp_avg_scale=torch.ones(blocks), exp_avg_sq_scale=torch.ones(blocks)) if bits == 8 else st
+
+    params = [torch.nn.Parameter(torch.zeros(n)) for n in (7, 70)]
+    opt = FlatAdamW(params, state_bits=bits)
+    saved = dict(opt.state_dict(), state={i: moments(p.detach(), 3) for i, p in enumerate(params)})
+    opt.load_state_dict(saved)
+    saved["state"][1]["step"] += 1
+    with pytest.raises(ValueError, match="steps"):
+        opt.load_state_dict(saved)
+    assert [float(opt.state[p]["step"]) for p in params] == [3, 3]
+    assert all((opt.state[p]["exp_avg"].float() == 1).all() for p in params)
