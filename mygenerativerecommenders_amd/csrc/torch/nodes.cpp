@@ -264,6 +264,9 @@ void adamw8_step(at::TensorList params, const Tensor& exp_avg, const Tensor& exp
                      fptr(exp_avg_scale), (uint8_t*)exp_avg_sq.data_ptr(), fptr(exp_avg_sq_scale), fptr(step),
                      (uint32_t*)counters.data_ptr(), lr, beta1, beta2, eps, weight_decay, stream(step)),
        "gr_adamw8_step");
+  // a graph that saved a parameter before must not go on with what it is now
+  for (size_t i = 0; i < n; ++i)
+    if (p[i]) params[i].unsafeGetTensorImpl()->bump_version();
 }
 
 }  // namespace

@@ -487,3 +487,16 @@ def test_goes_the_way_of_the_32_bit_optimizer():
         ends.append(p.detach().double())
     assert ends[1].norm() > 4
     assert abs((ends[0] @ ends[1] / ends[1].square().sum()).item() - 1) <= 0.25
+
+
+def test_a_step_shows_in_the_version_of_what_it_changed():
+    """A graph that saved a parameter before the step raises, as with torch's optimizers; one that saved a
+    parameter without a gradient does not."""
+    params, opt, g = make([(8,), (8,)], **HYPER)
+    gradients(params, g, 0)
+    params[1].grad = None
+    losses = [p.square().sum() for p in params]
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        losses[0].backward()
+    losses[1].backward()
