@@ -533,20 +533,26 @@ __device__ __forceinline__ float half_sum(float v) {
 template <typename T, int DP>
 constexpr bool ja_keep = sizeof(T) == 2 || DP <= 128;
 
-// Whether there are at most `per_cu` tiles of 128 rows for each CU.  The fewer the tiles, the
-// more wave sets share a workgroup's: the longest tile's time is what counts then, and with
-// many tiles the joining is only in the way.  Measured over ragged batches, bf16 (us):
-//   width 64, forward / dQ / key pass: 32 x 2,028 rows, 1 head (302 tiles): 4 sets of two waves 37 / 41 / 46, one
-//   set of four 49 / 61 / 64; 24 x 1,000, 2 heads (422): 37 / 41 / 46 and 30 / 36 / 39;
-//   width 128, forward: 2 x 8,192 rows, 4 heads (392): two sets 109, one 146; 24 x 980, 4 heads (488):
-//   42 and 40; 128 x 700, 4 heads (2,000): 117 and 87.
-// Key pass at width 128: 24 x 1,000 rows, 4 heads (488 tiles): two sets 44, one 62; 128 x 996, 8 heads on
-// one (653): 275 and 406; 200 x 100, 2 heads (712): 28 and 21; 128 x 996, 4 heads (2,612): 239 and 192.
+// Whether there are at most `per_cu` tiles of 128 rows for each CU: the buffers' rows / 128 and one for
+// each sequence, times heads.  (The offsets are not read on the host: spare rows count as tiles, and the
+// sequences' lengths, which decide too, do not show.)  The fewer the tiles, the more wave sets share a
+// workgroup's: the longest tile's time is what counts then, and with many tiles the joining is only in
+// the way.  Measured over ragged batches (lengths spread evenly up to the one given), causal, us of the
+// kernel, one set and more:
+//   bf16, width 64, forward: 24 x 1,000 rows, 2 heads (242 tiles) 27 and 20, 32 x 2,028, 1 head (295) 48 and 34,
+//   24 x 1,000, 4 heads (484) 30 and 38; dQ (width 62): 37 and 26, 67 and 44, 42 and 48; key pass: 34 and 24,
+//   62 and 42, 24 x 1,499, 8 heads on 2 (338) 171 and 96;
+//   width 128, forward: 2 x 8,192 rows, 4 heads (336 tiles) 234 and 182, 24 x 980, 4 heads (476) 38 and 37, 64 x
+//   1,000, 2 heads (650) 42 and 52; dQ: 306 and 193, 48 and 45, 50 and 62;
+//   fp32, width 64 (two sets and four), forward: 4 x 3,524 rows, 2 heads (130 tiles) 142 and 129, 128 x 211, 1 head
+//   (238) 17 and 19, 24 x 980, 4 heads (476) 58 and 68; key pass: 258 and 240, 30 and 28, 106 and 116.
+// Key pass at width 128: its bound lies where long sequences still gain and short ones lose, 24 x 1,000 rows,
+// 4 heads (484 tiles) 61 and 42, 200 x 100, 2 heads (562) 18 and 20, 128 x 996, 8 heads on 1 (650) 405 and 284, 64 x
+// 1,000, 2 heads (650) 66 and 60, 128 x 500, 2 heads (780) 44 and 50, 128 x 996, 4 heads (2,600) 200 and 224.
 // At width 256 a workgroup of two sets fills a CU's LDS and one of a single set half of it, and then
-// a SIMD has two waves (forward / dQ / key passes, us):
-//   32 x 2,028, 1 head (298 tiles): two sets 86 / 104 / 203, one set of four waves 117 / 135 / 313;
-//   24 x 1,000, 2 heads (422): 88 / 107 / 197 and 71 / 88 / 174; 128 x 996, 4 heads: 444 / 542 / 917
-//   and 263 / 455 / 640.
+// a SIMD has two waves.  Forward, 24 x 1,000 rows, 2 heads (242 tiles) 64 and 43, 32 x 2,028, 1 head (295) 117 and 81,
+// 128 x 996, 4 heads (2,600) 271 and 440; dQ (width 254): 85 and 57, 155 and 110, 24 x 1,000, 4 heads (484) 95 and
+// 107; key passes: 144 and 98, 272 and 177, 587 and 813.
 inline bool jagged_few(const JaggedAttnArgs& a, int heads, float per_cu) {
   return (float)((a.rows / 128 + a.B) * heads) <= per_cu * device_cus();
 }

@@ -8,10 +8,10 @@
 // rows (dK and dV, summed over the query heads that share them).  Seven products instead
 // of the five that one pass with atomic dQ sums would take (eight at widths above 128).
 //
-// bf16, 32 x 2,059 ragged rows, one head of 256: 263 us (alone dQ 104, dV 83, dK 104), one wave a
-// SIMD and bound by the longest sequence's chain of tiles.  24 x 1,499 rows, 8 heads on 2 of 64: 58 and 98.
-// 128 x 996 rows, 4 heads of 128: 201 and 195, two waves a SIMD.  fp32 runs at half the matrix rate:
-// 128 x 211 ragged rows, one head of 50: 46 us, of which some 16 are what one tile takes.
+// bf16, 32 x 2,059 ragged rows, one head of 256: 259 us and 10 for D, one wave a SIMD and bound by the longest
+// sequence's chain of tiles.  24 x 1,499 rows, 8 heads on 2 of 64: dQ 58, key pass 98.  128 x 996 rows, 4 heads of
+// 128: 213 and 216, two waves a SIMD.  fp32 products run at an eighth of bf16's rate: 128 x 211 ragged rows, one
+// head of 50: 36 us and 5 for D; a single sequence of 128 rows takes 16 and 4.
 #include <math.h>
 
 #include "jagged_attn.h"
@@ -272,11 +272,13 @@ __global__ __launch_bounds__(64 * QW * SETS, sizeof(T) == 2 && DP == 128 && (BYT
 
 // Few tiles: all passes in one launch, the key rows' workgroups first, after a launch for D.
 // Alone, each leaves CUs idle behind its longest tiles; with many, a pass would only have the
-// other's registers.  `keys` workgroups for each key pass.  In turn and joint (us), fp32 width 64:
-// 4 x 1,762 rows, 4 heads (144 tiles of 128 rows) 219 and 129, 128 x 211, 1 head (339) 62 and 55, 200 x 100,
-// 2 heads (712) 70 and 65; bf16 width 64: 32 x 2,028, 1 head (302) 82 and 74, 24 x 980, 4 heads (488)
-// 70 and 74; width 128: 144 tiles 102 and 60, 282 tiles 74 and 80; width 256: 144 tiles 214 and 147,
-// 302 274 and 263, 488 234 and 242.
+// other's registers.  `keys` workgroups for each key pass.  In turn and joint (us, the backward's kernels
+// together, causal ragged batches as at jagged_few):
+//   fp32, width 64: 128 x 211 rows, 1 head (238 tiles) 51 and 46, 4 x 3,524, 4 heads (260) 580 and 385, 64 x 500, 4 heads
+//   (776) 169 and 158; width 128: 81 and 65, 869 and 723, 347 and 332;
+//   bf16, width 64: 4 x 3,524, 4 heads (260) 156 and 96, 32 x 2,028, 1 head (295) 105 and 73, 24 x 980, 4 heads (476) 72 and 73;
+//   width 128: 8 x 2,400, 3 heads (243) 139 and 110, 32 x 2,028, 1 head (295) 124 and 112, 24 x 980, 4 heads (476) 86 and 108;
+//   width 256: 479 and 356, 32 x 2,059, 1 head (299) 312 and 255, 24 x 980, 4 heads (476) 226 and 227.
 template <typename T, int DP, int BN, int BYTES, int QW, int SETS>
 __global__ __launch_bounds__(64 * QW * SETS) void jagged_attn_both_kernel(JaggedAttnArgs a, unsigned keys) {
   __shared__ u32x4_t lds[SETS * 4 * JaTile<T, DP>::size(BN)];

@@ -11,9 +11,10 @@
 //
 // Bytes are no bound (q, k, v and out once: some 10 us where a launch takes 90); what is depends on
 // the tiles.  Few of them: the longest sequence's chain of tiles (2 x 8,192 rows, 4 heads of 128,
-// bf16: 137 us, 540 TFLOP/s).  Many: the vector work of the softmax, 16 exponentials a lane
+// bf16: 141 us, 526 TFLOP/s).  Many: the vector work of the softmax, 16 exponentials a lane
 // and tile beside 16 (width 64) to 64 matrix instructions, hidden only by other waves of the
-// SIMD (128 x 996 rows, 4 heads of 128: 156 us).  Tried and slower: the next tile's scores under this
+// SIMD (128 x 996 rows, 4 heads of 128: 110 us, 415 TFLOP/s; with
+// the rounding errors for a backward pass 168).  Tried and slower: the next tile's scores under this
 // tile's softmax in one wave (54 us -> 71, 213 -> 246), as the registers cost it a wave; tiles staged
 // through registers.
 #include <math.h>

@@ -1236,9 +1236,10 @@ def jagged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     row of its sequence and key head, those before it included, and no other.  Keys masked by a lowest
     value in a column of theirs are no part of a row that sees another key; a row whose largest scaled
     score is beyond 5.8e6 in magnitude (it sees masked keys alone, say) gives no gradient: its log-sum does
-    not hold in fp32.  Softmax and sums are fp32; bfloat16 probabilities enter the products
-    rounded to bfloat16, with their rounding errors as a second operand where a gradient is wanted
-    (so such outputs can differ in the last bit).  No atomics: the same bits every run.  Second and
+    not hold in fp32.  Softmax and sums are fp32; bfloat16 probabilities
+    (and, backward, their gradients) enter the products rounded to bfloat16; where a gradient is wanted, the
+    product with v takes their rounding errors as a second operand, so such outputs can differ in the last
+    bit.  No atomics: the same bits every run of the same sizes.  Second and
     forward-mode derivatives and traces raise."""
     _lib.require_gpu(q, k, v, offsets)
     if q.dtype not in _FLOATS or k.dtype != q.dtype or v.dtype != q.dtype:
