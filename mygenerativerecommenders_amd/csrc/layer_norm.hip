@@ -480,7 +480,8 @@ extern "C" {
 
 int gr_layer_norm_fwd(const void* x, int64_t ld_x, int64_t rows, int D, const void* weight, const void* bias,
                       int types, float eps, void* y, int64_t ld_y, float* stats, void* stream) {
-  GR_REQUIRE(rows >= 0 && D >= 1 && D < gr::LN_COLUMNS && types >= 0 && types < 4 && (rows == 0 || (x && y)), "gr_layer_norm_fwd: bad args");
+  GR_REQUIRE(rows >= 0 && D >= 1 && D < gr::LN_COLUMNS && types >= 0 && types < 4 && (rows == 0 || (x && y)),
+             "gr_layer_norm_fwd: bad args");
   GR_REQUIRE(rows <= 1 || ((ld_x >= D || ld_x == 0) && ld_y >= D), "gr_layer_norm_fwd: row strides below D");
   if (rows == 0) return 0;
   const hipStream_t st = (hipStream_t)stream;

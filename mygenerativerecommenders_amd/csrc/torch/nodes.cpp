@@ -2,7 +2,8 @@
 // (gr_amd::*).  A backward pass runs on one of torch's own threads: written in Python it takes
 // the interpreter there and back, some 45 us a call, more than the kernels of a small batch.
 // The C-ABI library is not linked: gr_torch_bind() takes the addresses of its functions, so that both
-// sides use the one that is loaded (no operator, or a trace that makes the first call would hold them).  Arguments are checked by the Python entry points.
+// sides use the one that is loaded (no operator, or a trace that makes the first call would hold
+// them).  Arguments are checked by the Python entry points.
 #include <ATen/ATen.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
@@ -48,9 +49,8 @@ Tensor floats(const Tensor& like, at::IntArrayRef size) { return at::empty(size,
 Tensor bytes(const Tensor& like, size_t n) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
 Tensor plain(const Tensor& like) { return at::empty(like.sizes(), like.options()); }
 
-// The kernels read memory and know nothing of forward-mode tangents, batched maps and traces: these raise
-// (they would go on without the operator).  Tensors of such kinds have no memory of their own or keys
-// of their own; a trace of plain tensors shows in its mode.
+// The kernels read memory: forward-mode tangents, transforms and traces would go on without the
+// operator, so they raise.  Wrapped tensors show by their dispatch keys, a trace of plain ones by its mode.
 bool has_tangent(const Tensor& t) {
   return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined();
 }

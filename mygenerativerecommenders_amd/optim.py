@@ -106,12 +106,15 @@ class FlatAdamW(torch.optim.Optimizer):
     def _fill(self, fs: dict, params: list) -> None:
         """Moves what ``self.state`` holds for the parameters (a loaded state, checked) into a group's
         buffers, zeros where they hold nothing yet, and makes the state views of them."""
+        step = None
         for p, off in zip(params, fs["offs"].tolist()):
             loaded, self.state[p] = self.state.get(p), self._views(fs, p, off)
             if loaded:
                 for n in self._names():
                     self.state[p][n].copy_(loaded[n])
-                fs["step"].copy_(torch.as_tensor(loaded["step"], dtype=torch.float32).reshape(1))
+                step = loaded["step"]
+        if step is not None:
+            fs["step"].copy_(torch.as_tensor(step, dtype=torch.float32).reshape(1))
 
     def flat_state(self, group: int = 0) -> dict:
         """The flat buffers behind a parameter group's per-parameter state, by torch's names
